@@ -1,0 +1,668 @@
+// apex_amd._token_loss — losses on the log-probabilities of given tokens.
+//
+// For a row x of logits (V values), its label y and a temperature T
+//   lp = x_y / T - log sum_v exp(x_v / T)
+// and for any loss of the lp with c = dloss/dlp
+//   dloss/dx_v = c ([v = y] - exp(x_v / T - lse)) / T.
+// So every loss here is a pass over the rows that keeps two floats of each
+// (its maximum m and log2 of sum exp((x - m) / T)), a small pass over the rows'
+// lp that makes the loss and c, and a backward pass that reads the logits again
+// and writes their gradient. Rows whose label is `ignore` are not read; their lp
+// is 0 and their gradient rows are 0. A label outside [0, V) reads nothing and
+// gives NaN.
+//
+// What bounds them: HBM. Forward reads the labelled rows once, backward reads
+// them once more and writes the whole gradient.
+#include "common.h"
+
+#include <c10/core/DeviceGuard.h>
+
+#include <cmath>
+#include <limits>
+#include <tuple>
+#include <vector>
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+// Rows of a tensor [.., V] whose leading dimensions come down to two.
+struct Rows {
+  long inner, outer_stride, inner_stride;  // row r is at (r / inner) * outer_stride + (r % inner) * inner_stride
+  __device__ __forceinline__ long at(long r) const {
+    return (r / inner) * outer_stride + (r % inner) * inner_stride;
+  }
+};
+
+// Sequences over the rows: `length` rows each, or rows [cu[s], cu[s + 1]) where cu is given.
+struct Sequences {
+  const int* cu;
+  long length, rows;
+  __device__ __forceinline__ void span(long s, long& begin, long& end) const {
+    if (cu) {  // the values cannot be looked at on the host without waiting: keep them inside the rows here
+      begin = min(max((long)cu[s], 0L), rows);
+      end = min(max((long)cu[s + 1], begin), rows);
+    } else {
+      begin = s * length;
+      end = begin + length;
+    }
+  }
+};
+
+template <typename T>
+struct Pack {
+  static constexpr int width = 16 / sizeof(T);
+  T a[width];
+};
+
+// 16 bytes from an address that is aligned to its element only (rows of an odd V)
+template <typename T>
+__device__ __forceinline__ Pack<T> load16(const T* p) {
+  Pack<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const Pack<T>& v) {
+  __builtin_memcpy(p, &v, 16);
+}
+
+// m = max x, s = sum exp2((x - m) c), over what has been added
+struct Running {
+  float m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ void raise(float top, float c) {
+    if (top > m) {
+      s *= __builtin_amdgcn_exp2f((m - top) * c);  // m = -inf: s is 0 and stays so
+      m = top;
+    }
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    // an m of -inf has no differences: against 0, exp2 of -inf is 0
+    s += __builtin_amdgcn_exp2f((x - (m == -INFINITY ? 0.f : m)) * c);
+  }
+  __device__ __forceinline__ void join(float mb, float sb, float c) {
+    const float top = fmaxf(m, mb), against = top == -INFINITY ? 0.f : top;
+    s = s * __builtin_amdgcn_exp2f((m - against) * c) + sb * __builtin_amdgcn_exp2f((mb - against) * c);
+    m = top;
+  }
+};
+
+template <int BLOCK>
+__device__ __forceinline__ Running block_join(Running w, float c, float* smem) {
+#pragma unroll
+  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1)
+    w.join(__shfl_xor(w.m, off), __shfl_xor(w.s, off), c);
+  constexpr int NW = BLOCK / WAVE_SIZE;
+  if ((threadIdx.x & (WAVE_SIZE - 1)) == 0) {
+    smem[2 * (threadIdx.x / WAVE_SIZE)] = w.m;
+    smem[2 * (threadIdx.x / WAVE_SIZE) + 1] = w.s;
+  }
+  __syncthreads();
+  Running all;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) all.join(smem[2 * i], smem[2 * i + 1], c);
+  return all;
+}
+
+// A block's sum in 64 bits, in a fixed order; valid on every thread.
+template <int BLOCK>
+__device__ __forceinline__ double block_sum(double v, double* smem) {
+#pragma unroll
+  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  constexpr int NW = BLOCK / WAVE_SIZE;
+  __syncthreads();
+  if ((threadIdx.x & (WAVE_SIZE - 1)) == 0) smem[threadIdx.x / WAVE_SIZE] = v;
+  __syncthreads();
+  double all = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) all += smem[i];
+  return all;
+}
+
+// ---------------- rows: maximum, sum and log-probability ----------------
+template <typename T, int BLOCK>
+__global__ void __launch_bounds__(BLOCK) row_stats_kernel(
+    const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
+    long rows, float c, float2* __restrict__ stats, float* __restrict__ lp_out, int* __restrict__ arrived) {
+  __shared__ float smem[2 * (BLOCK / WAVE_SIZE)];
+  constexpr int W = Pack<T>::width;
+  if (arrived && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // for the kernel after this one
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+  const long y = labels[row];
+  if (y == ignore || y < 0 || y >= V) {
+    if (threadIdx.x == 0) {
+      const float none = y == ignore ? 0.f : NAN;
+      lp_out[row] = none;
+      stats[row] = make_float2(none, none);
+    }
+    continue;
+  }
+  const T* x = logits + where.at(row);
+  Running w;
+  const long whole = V / W;
+  for (long k = threadIdx.x; k < whole; k += BLOCK) {
+    const Pack<T> v = load16(x + k * W);
+    float top = to_float(v.a[0]);
+#pragma unroll
+    for (int j = 1; j < W; ++j) top = fmaxf(top, to_float(v.a[j]));
+    w.raise(top, c);
+#pragma unroll
+    for (int j = 0; j < W; ++j) w.add(to_float(v.a[j]), c);
+  }
+  for (long i = whole * W + threadIdx.x; i < V; i += BLOCK) {
+    const float f = to_float(x[i]);
+    w.raise(f, c);
+    w.add(f, c);
+  }
+  w = block_join<BLOCK>(w, c, smem);
+  if (threadIdx.x == 0) {
+    const float l2 = log2f(w.s);
+    lp_out[row] = ((to_float(x[y]) - w.m) * c - l2) * LN2;
+    stats[row] = make_float2(w.m, l2);
+  }
+  __syncthreads();  // smem is the next row's
+  }
+}
+
+// ---------------- rows: gradient ----------------
+// coef[r] (with `scale` and `norm`, where given) is the gradient of row r's lp.
+template <typename T, int BLOCK>
+__global__ void __launch_bounds__(BLOCK) row_grad_kernel(
+    const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
+    long rows, float c, float inv_t, const float2* __restrict__ stats, const float* __restrict__ coef,
+    const float* __restrict__ scale, long scale_stride, const float* __restrict__ norm,
+    T* __restrict__ grad) {
+  constexpr int W = Pack<T>::width;
+  const long whole = V / W;
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+  const long y = labels[row];
+  T* g = grad + row * V;
+  if (y == ignore) {
+    Pack<T> zero;
+#pragma unroll
+    for (int j = 0; j < W; ++j) zero.a[j] = from_float<T>(0.f);
+    for (long k = threadIdx.x; k < whole; k += BLOCK) store16(g + k * W, zero);
+    for (long i = whole * W + threadIdx.x; i < V; i += BLOCK) g[i] = from_float<T>(0.f);
+    continue;
+  }
+  const T* x = logits + where.at(row);
+  const float2 st = stats[row];
+  float f = coef[row] * inv_t;
+  if (scale) f *= scale[row * scale_stride];
+  if (norm) f *= *norm;
+  for (long k = threadIdx.x; k < whole; k += BLOCK) {
+    const Pack<T> v = load16(x + k * W);
+    Pack<T> o;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(to_float(v.a[j]) - st.x, c, -st.y));
+      o.a[j] = from_float<T>(f * ((k * W + j == y ? 1.f : 0.f) - p));
+    }
+    store16(g + k * W, o);
+  }
+  for (long i = whole * W + threadIdx.x; i < V; i += BLOCK) {
+    const float p = __builtin_amdgcn_exp2f(fmaf(to_float(x[i]) - st.x, c, -st.y));
+    g[i] = from_float<T>(f * ((i == y ? 1.f : 0.f) - p));
+  }
+  }
+}
+
+// ---------------- sequences ----------------
+constexpr int SEQ_BLOCK = 256;
+
+// Sum (in 64 bits) and number of a sequence's labelled lp.
+__device__ __forceinline__ void sum_span(const float* lp, const long* labels, long ignore, long begin,
+                                         long end, double* smem, double& sum, double& count) {
+  double s = 0, n = 0;
+  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) {
+    const bool on = labels[r] != ignore;
+    s += on ? (double)lp[r] : 0.0;
+    n += on ? 1.0 : 0.0;
+  }
+  sum = block_sum<SEQ_BLOCK>(s, smem);
+  count = block_sum<SEQ_BLOCK>(n, smem);
+}
+
+__global__ void __launch_bounds__(SEQ_BLOCK) sequence_sum_kernel(
+    const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
+    bool average, float* __restrict__ out) {
+  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  long begin, end;
+  seqs.span(blockIdx.x, begin, end);
+  double sum, count;
+  sum_span(lp, labels, ignore, begin, end, smem, sum, count);
+  if (threadIdx.x == 0) out[blockIdx.x] = (float)(average ? sum / fmax(count, 1.0) : sum);
+}
+
+// coef of each row of a sequence from the gradient of the sequence's sum
+__global__ void __launch_bounds__(SEQ_BLOCK) sequence_coef_kernel(
+    const float* __restrict__ grad, const long* __restrict__ labels, long ignore, Sequences seqs,
+    bool average, float* __restrict__ coef) {
+  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  long begin, end;
+  seqs.span(blockIdx.x, begin, end);
+  double n = 0;
+  if (average)
+    for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) n += labels[r] != ignore ? 1.0 : 0.0;
+  n = block_sum<SEQ_BLOCK>(n, smem);
+  const float f = average ? (float)(grad[blockIdx.x] / fmax(n, 1.0)) : grad[blockIdx.x];
+  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) coef[r] = f;
+}
+
+// True on the block that comes last, on all its threads; what the others wrote before is then visible to it.
+__device__ __forceinline__ bool comes_last(int* arrived, int blocks, int* smem) {
+  if (threadIdx.x == 0) {
+    __threadfence();
+    *smem = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  return *smem != 0;
+}
+
+__device__ __forceinline__ double read_shared(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---------------- paired log ratios ----------------
+// One block a pair: sequence b was chosen, sequence pairs + b rejected. With
+// d = (S_chosen - R_chosen) - (S_rejected - R_rejected), S and R the sequences'
+// log-probabilities under the policy and the reference:
+//   sigmoid: -(1 - e) log sigmoid(beta d) - e log sigmoid(-beta d)
+//   ipo:     (d - 1 / (2 beta))^2
+//   hinge:   max(0, 1 - beta d)
+// The sums and d are kept in 64 bits: d is a small difference of large sums.
+enum { SIGMOID = 0, IPO = 1, HINGE = 2 };
+
+__global__ void __launch_bounds__(SEQ_BLOCK) preference_kernel(
+    const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
+    const float* __restrict__ ref, long pairs, int kind, double beta, double smoothing, bool average,
+    float* __restrict__ coef, float* __restrict__ rewards, double* __restrict__ partial,
+    int* __restrict__ arrived, float* __restrict__ loss_out) {
+  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  __shared__ int last;
+  const long b = blockIdx.x;
+  long begin[2], end[2];
+  double sum[2], count[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    seqs.span(b + k * pairs, begin[k], end[k]);
+    sum_span(lp, labels, ignore, begin[k], end[k], smem, sum[k], count[k]);
+    count[k] = average ? fmax(count[k], 1.0) : 1.0;
+  }
+  const double chosen = sum[0] / count[0] - (double)ref[b];
+  const double rejected = sum[1] / count[1] - (double)ref[b + pairs];
+  const double d = chosen - rejected, z = beta * d;
+  double loss, slope;  // slope = dloss/dd
+  if (kind == SIGMOID) {
+    // log(1 + exp(-z)) without an exp that overflows
+    const double e = exp(-fabs(z)), soft = log1p(e);
+    const double minus = fmax(-z, 0.0) + soft, plus = fmax(z, 0.0) + soft;
+    const double up = (z >= 0 ? e : 1.0) / (1.0 + e);  // sigmoid(-z)
+    loss = (1.0 - smoothing) * minus + smoothing * plus;
+    slope = beta * (smoothing * (1.0 - up) - (1.0 - smoothing) * up);
+  } else if (kind == IPO) {
+    const double off = d - 0.5 / beta;
+    loss = off * off;
+    slope = 2.0 * off;
+  } else {
+    loss = z >= 1.0 ? 0.0 : 1.0 - z;  // NaN stays NaN
+    slope = z >= 1.0 ? 0.0 : -beta;
+  }
+  slope = z != z ? z : slope;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float f = (float)((k ? -slope : slope) / (count[k] * (double)pairs));
+    for (long r = begin[k] + threadIdx.x; r < end[k]; r += SEQ_BLOCK) coef[r] = f;
+  }
+  if (threadIdx.x == 0) {
+    rewards[b] = (float)(beta * chosen);
+    rewards[b + pairs] = (float)(beta * rejected);
+    partial[b] = loss;
+  }
+  if (!comes_last(arrived, gridDim.x, &last)) return;
+  double total = 0;
+  for (long i = threadIdx.x; i < pairs; i += SEQ_BLOCK) total += read_shared(partial + i);
+  total = block_sum<SEQ_BLOCK>(total, smem);
+  if (threadIdx.x == 0) *loss_out = (float)(total / (double)pairs);
+}
+
+// ---------------- clipped policy loss ----------------
+// With ratio = exp(lp - old), advantage A and d = ref - lp:
+//   loss = -min(ratio A, clamp(ratio, 1 - low, 1 + high) A) + kl (exp(d) - d - 1)
+//   dloss/dlp = (-ratio A where the minimum is the unclipped one) - kl (exp(d) - 1)
+struct Policy {
+  const float *old, *ref, *advantages;
+  bool by_row;  // an advantage for each row, or for each sequence
+  float low, high, kl;
+  __device__ __forceinline__ float of(float lp, long r, long s, float& slope) const {
+    const float a = advantages[by_row ? r : s];
+    const float ratio = old ? expf(lp - old[r]) : (lp == lp ? 1.f : lp);
+    const float held = ratio < 1.f - low ? 1.f - low : ratio > 1.f + high ? 1.f + high : ratio;
+    float loss = -(ratio * a > held * a ? held * a : ratio * a);
+    slope = ratio * a > held * a ? 0.f : -ratio * a;
+    if (ref) {
+      const float d = ref[r] - lp, grown = expm1f(d);
+      loss = fmaf(kl, grown - d, loss);
+      slope = fmaf(-kl, grown, slope);
+    }
+    return loss;
+  }
+};
+
+enum { TOKEN = 0, SEQUENCE = 1, SUM = 2, NONE = 3 };
+
+// One block a sequence. `coef` comes without the division by the number of all
+// tokens (TOKEN): that number is known at the end only and goes out as `norm`.
+__global__ void __launch_bounds__(SEQ_BLOCK) policy_kernel(
+    const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
+    Policy policy, int reduction, float* __restrict__ coef, float* __restrict__ losses,
+    double* __restrict__ partial, int* __restrict__ arrived, float* __restrict__ norm,
+    float* __restrict__ loss_out) {
+  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  __shared__ int last;
+  const long s = blockIdx.x;
+  long begin, end;
+  seqs.span(s, begin, end);
+  double n = 0, sum = 0;
+  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) n += labels[r] != ignore ? 1.0 : 0.0;
+  n = block_sum<SEQ_BLOCK>(n, smem);
+  const double weight = reduction == SEQUENCE ? 1.0 / (fmax(n, 1.0) * (double)gridDim.x) : 1.0;
+  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) {
+    float loss = 0.f, slope = 0.f;
+    if (labels[r] != ignore) loss = policy.of(lp[r], r, s, slope);
+    coef[r] = (float)(weight * slope);
+    if (reduction == NONE) losses[r] = loss;
+    sum += weight * loss;
+  }
+  if (reduction == NONE) return;
+  sum = block_sum<SEQ_BLOCK>(sum, smem);
+  if (threadIdx.x == 0) {
+    partial[2 * s] = sum;
+    partial[2 * s + 1] = n;
+  }
+  if (!comes_last(arrived, gridDim.x, &last)) return;
+  double total = 0, tokens = 0;
+  for (long i = threadIdx.x; i < gridDim.x; i += SEQ_BLOCK) {
+    total += read_shared(partial + 2 * i);
+    tokens += read_shared(partial + 2 * i + 1);
+  }
+  total = block_sum<SEQ_BLOCK>(total, smem);
+  tokens = block_sum<SEQ_BLOCK>(tokens, smem);
+  if (threadIdx.x == 0) {
+    const double by = reduction == TOKEN ? 1.0 / fmax(tokens, 1.0) : 1.0;
+    *norm = (float)by;
+    *loss_out = (float)(total * by);
+  }
+}
+
+// What the gradient is multiplied by, of a number and a value on the device.
+__global__ void scale_kernel(float number, const float* __restrict__ value, float* __restrict__ applied) {
+  *applied = value ? number * *value : number;
+}
+
+// A gradient made for `applied` becomes that for *scale. Most often they are the same and nothing is moved.
+template <typename T>
+__global__ void __launch_bounds__(256) rescale_kernel(T* __restrict__ grad, long n, const float* __restrict__ scale,
+                                                      const float* __restrict__ applied) {
+  const float a = *applied, b = *scale;
+  if (a == b) return;
+  const float f = b / a;
+  constexpr int W = Pack<T>::width;
+  const long step = (long)gridDim.x * 256, whole = n / W, first = blockIdx.x * 256L + threadIdx.x;
+  for (long k = first; k < whole; k += step) {
+    Pack<T> v = load16(grad + k * W);
+#pragma unroll
+    for (int j = 0; j < W; ++j) v.a[j] = from_float<T>(to_float(v.a[j]) * f);
+    store16(grad + k * W, v);
+  }
+  for (long i = whole * W + first; i < n; i += step) grad[i] = from_float<T>(to_float(grad[i]) * f);
+}
+
+// ---------------- host ----------------
+Rows rows_of(at::Tensor& x) {
+  // merges leading dimensions that lie evenly; copies what does not come down to two
+  for (int pass = 0; pass < 2; ++pass) {
+    std::vector<std::pair<long, long>> dims;  // (size, stride), outermost first
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) {
+      if (x.size(d) == 1) continue;
+      if (!dims.empty() && dims.back().second == x.stride(d) * x.size(d))
+        dims.back() = {dims.back().first * x.size(d), x.stride(d)};
+      else
+        dims.push_back({x.size(d), x.stride(d)});
+    }
+    if (dims.size() <= 2 && (x.stride(-1) == 1 || x.size(-1) == 1)) {
+      if (dims.empty()) return {1, 0, 0};
+      if (dims.size() == 1) return {dims[0].first, 0, dims[0].second};
+      return {dims[1].first, dims[0].second, dims[1].second};
+    }
+    x = x.contiguous();
+  }
+  TORCH_CHECK(false, "token_loss: logits do not come down to rows");
+}
+
+// a launch's threads are counted in 32 bits: further rows are taken in turns
+unsigned grid_of(long rows) { return (unsigned)std::min<long>(rows, 1 << 20); }
+
+void check_rows(const at::Tensor& logits, const at::Tensor& labels) {
+  TORCH_CHECK(logits.is_cuda(), "token_loss: logits must be on the GPU");
+  TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) > 0, "token_loss: logits need a last dimension of the vocabulary");
+  TORCH_CHECK(labels.scalar_type() == at::kLong, "token_loss: labels must be int64");
+  TORCH_CHECK(labels.device() == logits.device(), "token_loss: labels are on another device than the logits");
+  TORCH_CHECK(labels.is_contiguous(), "token_loss: labels must be contiguous");
+  TORCH_CHECK(labels.numel() * logits.size(-1) == logits.numel(), "token_loss: one label a row");
+  TORCH_CHECK(labels.numel() < std::numeric_limits<int>::max(), "token_loss: too many rows");
+}
+
+// fp32 and contiguous, on the logits' device, with n values
+const float* floats(const at::Tensor& t, const at::Tensor& logits, int64_t n, const char* name) {
+  TORCH_CHECK(t.device() == logits.device(), "token_loss: ", name, " is on another device than the logits");
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous(), "token_loss: ", name, " must be contiguous fp32");
+  TORCH_CHECK(t.numel() == n, "token_loss: ", name, " has ", t.numel(), " values, not ", n);
+  return t.data_ptr<float>();
+}
+
+Sequences sequences_of(const at::Tensor& labels, const c10::optional<at::Tensor>& cu, long count) {
+  TORCH_CHECK(count < (1 << 22), "token_loss: too many sequences");
+  Sequences s{nullptr, count ? labels.numel() / count : 0, labels.numel()};
+  if (cu) {
+    TORCH_CHECK(cu->device() == labels.device() && cu->scalar_type() == at::kInt && cu->is_contiguous(),
+                "token_loss: cu_seqlens must be contiguous int32 on the logits' device");
+    TORCH_CHECK(cu->numel() == count + 1, "token_loss: cu_seqlens has one value more than sequences");
+    s.cu = cu->data_ptr<int>();
+  } else {
+    TORCH_CHECK(count > 0 && labels.numel() % count == 0, "token_loss: rows do not divide into sequences");
+  }
+  return s;
+}
+
+void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, double temperature,
+                  float2* stats, float* lp, int* arrived) {
+  const Rows where = rows_of(logits);
+  const long V = logits.size(-1), rows = labels.numel();
+  APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
+    constexpr int BLOCK = 256;
+    hipLaunchKernelGGL((row_stats_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
+                       (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
+                       (float)(1.4426950408889634 / temperature), stats, lp, arrived);
+  }()));
+  HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace
+
+// -> (lp, stats): stats [rows, 2] is what the backward pass needs of each row
+std::tuple<at::Tensor, at::Tensor> token_forward(at::Tensor logits, at::Tensor labels, long ignore,
+                                                 double temperature) {
+  check_rows(logits, labels);
+  const at::DeviceGuard guard(logits.device());
+  auto opts = logits.options().dtype(at::kFloat);
+  auto lp = at::empty(labels.sizes(), opts);
+  auto stats = at::empty({labels.numel(), 2}, opts);
+  if (labels.numel())
+    launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), nullptr);
+  return {lp, stats};
+}
+
+at::Tensor rows_backward(at::Tensor logits, at::Tensor labels, at::Tensor stats, at::Tensor coef,
+                         c10::optional<at::Tensor> scale, c10::optional<at::Tensor> norm, long ignore,
+                         double temperature) {
+  check_rows(logits, labels);
+  const at::DeviceGuard guard(logits.device());
+  const long rows = labels.numel(), V = logits.size(-1);
+  auto grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  if (!rows) return grad;
+  const Rows where = rows_of(logits);
+  const float* st = floats(stats, logits, 2 * rows, "stats");
+  const float* co = floats(coef, logits, rows, "coef");
+  const float* sc = scale ? floats(*scale, logits, scale->numel() == 1 ? 1 : rows, "grad_output") : nullptr;
+  const float* no = norm ? floats(*norm, logits, 1, "norm") : nullptr;
+  const long step = scale && scale->numel() == rows && rows > 1 ? 1 : 0;
+  APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
+    constexpr int BLOCK = 256;
+    hipLaunchKernelGGL((row_grad_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
+                       (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
+                       (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature),
+                       (const float2*)st, co, sc, step, no, (scalar_t*)grad.data_ptr());
+  }()));
+  HIP_CHECK(hipGetLastError());
+  return grad;
+}
+
+// -> (sums, stats)
+std::tuple<at::Tensor, at::Tensor> sequence_forward(at::Tensor logits, at::Tensor labels,
+                                                    c10::optional<at::Tensor> cu, long count, bool average,
+                                                    long ignore, double temperature) {
+  check_rows(logits, labels);
+  const at::DeviceGuard guard(logits.device());
+  auto opts = logits.options().dtype(at::kFloat);
+  const Sequences seqs = sequences_of(labels, cu, count);
+  auto lp = at::empty(labels.sizes(), opts);
+  auto stats = at::empty({labels.numel(), 2}, opts);
+  auto out = at::empty({count}, opts);
+  if (labels.numel())
+    launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), nullptr);
+  if (count)
+    hipLaunchKernelGGL(sequence_sum_kernel, dim3(count), dim3(SEQ_BLOCK), 0, current_stream(),
+                       lp.data_ptr<float>(), labels.data_ptr<long>(), ignore, seqs, average, out.data_ptr<float>());
+  HIP_CHECK(hipGetLastError());
+  return {out, stats};
+}
+
+at::Tensor sequence_coef(at::Tensor grad, at::Tensor labels, c10::optional<at::Tensor> cu, bool average, long ignore) {
+  const at::DeviceGuard guard(labels.device());
+  const long count = grad.numel();
+  const Sequences seqs = sequences_of(labels, cu, count);
+  const float* g = floats(grad, labels, count, "grad_output");
+  // rows behind the last packed sequence belong to none and get 0
+  auto coef = cu ? at::zeros(labels.sizes(), grad.options()) : at::empty(labels.sizes(), grad.options());
+  if (count)
+    hipLaunchKernelGGL(sequence_coef_kernel, dim3(count), dim3(SEQ_BLOCK), 0, current_stream(), g,
+                       labels.data_ptr<long>(), ignore, seqs, average, coef.data_ptr<float>());
+  HIP_CHECK(hipGetLastError());
+  return coef;
+}
+
+// -> (loss, rewards [2 pairs], stats, coef)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_forward(
+    at::Tensor logits, at::Tensor labels, at::Tensor ref, c10::optional<at::Tensor> cu, long pairs, long kind,
+    double beta, double smoothing, bool average, long ignore) {
+  check_rows(logits, labels);
+  const at::DeviceGuard guard(logits.device());
+  TORCH_CHECK(labels.numel() > 0 && pairs > 0, "preference_loss: needs a pair and a row");
+  const Sequences seqs = sequences_of(labels, cu, 2 * pairs);
+  const float* rf = floats(ref, logits, 2 * pairs, "ref_log_probs");
+  const long rows = labels.numel();
+  auto opts = logits.options().dtype(at::kFloat);
+  auto lp = at::empty({rows}, opts);
+  auto stats = at::empty({rows, 2}, opts);
+  auto coef = cu ? at::zeros({rows}, opts) : at::empty({rows}, opts);
+  auto rewards = at::empty({2 * pairs}, opts);
+  auto loss = at::empty({}, opts);
+  auto partial = at::empty({pairs + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
+  int* arrived = (int*)(partial.data_ptr<double>() + pairs);
+  launch_stats(logits, labels, ignore, 1.0, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), arrived);
+  hipLaunchKernelGGL(preference_kernel, dim3(pairs), dim3(SEQ_BLOCK), 0, current_stream(), lp.data_ptr<float>(),
+                     labels.data_ptr<long>(), ignore, seqs, rf, pairs, (int)kind, beta, smoothing, average,
+                     coef.data_ptr<float>(), rewards.data_ptr<float>(), partial.data_ptr<double>(), arrived,
+                     loss.data_ptr<float>());
+  HIP_CHECK(hipGetLastError());
+  return {loss, rewards, stats, coef};
+}
+
+// -> (loss, lp, stats, coef, norm)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_forward(
+    at::Tensor logits, at::Tensor labels, c10::optional<at::Tensor> old, at::Tensor advantages,
+    bool by_row, c10::optional<at::Tensor> ref, c10::optional<at::Tensor> cu, long count, double low, double high,
+    double kl, double temperature, long reduction, long ignore) {
+  check_rows(logits, labels);
+  const at::DeviceGuard guard(logits.device());
+  const long rows = labels.numel();
+  TORCH_CHECK(rows > 0 && count > 0, "policy_loss: needs a sequence and a row");
+  const Sequences seqs = sequences_of(labels, cu, count);
+  Policy policy{old ? floats(*old, logits, rows, "old_log_probs") : nullptr,
+                ref ? floats(*ref, logits, rows, "ref_log_probs") : nullptr,
+                floats(advantages, logits, by_row ? rows : count, "advantages"), by_row, (float)low, (float)high,
+                (float)kl};
+  auto opts = logits.options().dtype(at::kFloat);
+  auto lp = at::empty(labels.sizes(), opts);
+  auto stats = at::empty({rows, 2}, opts);
+  // rows behind the last packed sequence belong to none: no loss, no gradient
+  auto coef = cu ? at::zeros({rows}, opts) : at::empty({rows}, opts);
+  auto norm = at::empty({1}, opts);
+  at::Tensor loss;
+  if (reduction == NONE) loss = cu ? at::zeros(labels.sizes(), opts) : at::empty(labels.sizes(), opts);
+  else loss = at::empty({}, opts);
+  auto partial = at::empty({2 * count + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
+  int* arrived = (int*)(partial.data_ptr<double>() + 2 * count);
+  launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), arrived);
+  hipLaunchKernelGGL(policy_kernel, dim3(count), dim3(SEQ_BLOCK), 0, current_stream(), lp.data_ptr<float>(),
+                     labels.data_ptr<long>(), ignore, seqs, policy, (int)reduction, coef.data_ptr<float>(),
+                     loss.data_ptr<float>(), partial.data_ptr<double>(), arrived, norm.data_ptr<float>(),
+                     loss.data_ptr<float>());
+  HIP_CHECK(hipGetLastError());
+  return {loss, lp, stats, coef, norm};
+}
+
+// The gradient is made here, for a gradient of the loss that is known -> (loss, lp, dlogits, applied)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
+    at::Tensor logits, at::Tensor labels, c10::optional<at::Tensor> old, at::Tensor advantages, bool by_row,
+    c10::optional<at::Tensor> ref, c10::optional<at::Tensor> cu, long count, double low, double high, double kl,
+    double temperature, long reduction, long ignore, double scale, c10::optional<at::Tensor> scale_tensor) {
+  check_rows(logits, labels);
+  const at::DeviceGuard guard(logits.device());
+  auto applied = at::empty({1}, logits.options().dtype(at::kFloat));
+  const float* value = scale_tensor ? floats(*scale_tensor, logits, 1, "grad_scale") : nullptr;
+  hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1), 0, current_stream(), (float)scale, value, applied.data_ptr<float>());
+  auto [loss, lp, stats, coef, norm] = policy_forward(logits, labels, old, advantages, by_row, ref, cu, count, low, high,
+                                                      kl, temperature, reduction, ignore);
+  auto grad = rows_backward(logits, labels, stats, coef, applied, norm, ignore, temperature);
+  return {loss, lp, grad, applied};
+}
+
+void rescale_(at::Tensor grad, at::Tensor scale, at::Tensor applied) {
+  const at::DeviceGuard guard(grad.device());
+  TORCH_CHECK(grad.is_contiguous(), "rescale_: the gradient must be contiguous");
+  const float *s = floats(scale, grad, 1, "grad_output"), *a = floats(applied, grad, 1, "applied");
+  const long n = grad.numel();
+  if (!n) return;
+  const unsigned grid = (unsigned)std::min<long>((n + 2047) / 2048, 2048);
+  APEX_DISPATCH_FLOAT_HALF_BF(grad.scalar_type(), "rescale_", ([&] {
+    hipLaunchKernelGGL((rescale_kernel<scalar_t>), dim3(grid), dim3(256), 0, current_stream(),
+                       (scalar_t*)grad.data_ptr(), n, s, a);
+  }()));
+  HIP_CHECK(hipGetLastError());
+}
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("token_forward", &token_forward, "log-probabilities of given tokens -> (lp, stats)");
+  m.def("rows_backward", &rows_backward, "logits' gradient from that of the log-probabilities");
+  m.def("sequence_forward", &sequence_forward, "sequences' log-probabilities -> (sums, stats)");
+  m.def("sequence_coef", &sequence_coef, "gradient of each token from that of its sequence");
+  m.def("preference_forward", &preference_forward, "paired log ratios -> (loss, rewards, stats, coef)");
+  m.def("policy_forward", &policy_forward, "clipped policy loss with KL -> (loss, lp, stats, coef, norm)");
+  m.def("policy_at_once", &policy_at_once, "the policy loss and the logits' gradient -> (loss, lp, dlogits, applied)");
+  m.def("rescale_", &rescale_, "a gradient made for one gradient of the loss becomes that for another");
+}
