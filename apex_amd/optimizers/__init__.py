@@ -1,4 +1,5 @@
 from .fused_adam import FusedAdam
+from .fused_adam_8bit import FusedAdam8bit
 from .fused_sgd import FusedSGD
 from .fused_lamb import FusedLAMB
 from .fused_novograd import FusedNovoGrad
@@ -7,6 +8,7 @@ from .fused_mixed_precision_lamb import FusedMixedPrecisionLamb
 
 __all__ = [
     "FusedAdam",
+    "FusedAdam8bit",
     "FusedSGD",
     "FusedLAMB",
     "FusedNovoGrad",

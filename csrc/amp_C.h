@@ -52,6 +52,15 @@ void multi_tensor_adam_capturable_master_cuda(long chunk_size, at::Tensor noop_f
                                               at::Tensor step, long mode, long bias_correction,
                                               double weight_decay, at::Tensor inv_scale);
 
+void multi_tensor_adam_8bit_cuda(TensorLists tensor_lists, std::vector<long> ordinals, double lr, double beta1,
+                                 double beta2, double eps, long step, long mode, long bias_correction,
+                                 double weight_decay, long seed);
+
+void multi_tensor_adam_8bit_capturable_cuda(TensorLists tensor_lists, std::vector<long> ordinals, at::Tensor lr,
+                                            double beta1, double beta2, double eps, at::Tensor step, long mode,
+                                            long bias_correction, double weight_decay, long seed,
+                                            c10::optional<at::Tensor> inv_scale, c10::optional<at::Tensor> found_inf);
+
 void multi_tensor_adagrad_cuda(long chunk_size, at::Tensor noop_flag, TensorLists tensor_lists,
                                double lr, double eps, long mode, double weight_decay);
 

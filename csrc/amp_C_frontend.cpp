@@ -26,6 +26,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "hipGraph-capturable Adam (device lr/step/inv_scale)");
   m.def("multi_tensor_adam_capturable_master", &multi_tensor_adam_capturable_master_cuda,
         "hipGraph-capturable Adam with fp32 master params");
+  m.def("multi_tensor_adam_8bit", &multi_tensor_adam_8bit_cuda,
+        "Fused Adam/AdamW with both moments in 8 bits");
+  m.def("multi_tensor_adam_8bit_capturable", &multi_tensor_adam_8bit_capturable_cuda,
+        "hipGraph-capturable Adam with both moments in 8 bits");
   m.def("multi_tensor_adagrad", &multi_tensor_adagrad_cuda, "Fused Adagrad");
   m.def("multi_tensor_novograd", &multi_tensor_novograd_cuda,
         "Fused NovoGrad (per-tensor second moment vector)");

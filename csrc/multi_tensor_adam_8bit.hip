@@ -1,0 +1,396 @@
+// multi_tensor_adam_8bit — Adam/AdamW over many tensors with both moments in 8 bits.
+//
+// Mathematics. A moment is kept in blocks of 128 elements, in memory order from
+// the tensor's start: one fp32 scale s = max|x| / 448 and codes q in e4m3 (OCP,
+// 448 the largest), x = s q. The second moment v is kept as its root r, which
+// halves the octaves that its values span (a block holds r down to 2^-17 of its
+// largest). The step itself is in fp32 from the unrounded new moments.
+//   m = b1 m + (1 - b1) g,  v = b2 r^2 + (1 - b2) g^2
+//   p -= lr (m / bc1 / (sqrt(v) / sqrt(bc2) + eps) + wd p)
+//
+// Rounding. A step of b2 = 0.999 moves r by 0.05% a step where neighbouring codes
+// are 6 to 12% apart: rounded to nearest, r would never move. So a value becomes
+// the code below or above it at random, with odds that keep the mean of m, and of
+// v (not of r): P(above) = (x - lo) / (hi - lo), and (r^2 - lo^2) / (hi^2 - lo^2).
+// An r over 0 never becomes 0, for its inverse is used. The random numbers are a
+// hash of (seed, step, tensor, element): 16 bits for m, 16 for v. A run repeats
+// bit for bit, whatever the launch.
+// A value that is not finite becomes the code NaN in its place alone: a block's
+// scale is of its finite values.
+//
+// What bounds it: HBM. Per element of fp32 weights 12 B (g, p in and out) + 4 B
+// of moments + 0.125 B of scales, against 28 B with fp32 moments.
+#include "amp_C.h"
+#include "multi_tensor_apply.h"
+
+#include <c10/core/DeviceGuard.h>
+
+#include <cmath>
+
+namespace {
+
+constexpr int A8_BLOCK = 256;          // threads
+constexpr int A8_PER_LANE = 8;         // elements: 16 lanes have a block of 128
+constexpr int A8_SCALE_BLOCK = 128;    // elements of one scale
+constexpr int A8_CHUNK = 8192;         // elements of a workgroup
+constexpr int A8_TENSORS = 48;         // of one launch: 48 * 76 B of kernel arguments
+constexpr float E4M3_MAX = 448.f;
+
+struct Adam8Meta {
+  void* g[A8_TENSORS];
+  void* p[A8_TENSORS];
+  void* master[A8_TENSORS];
+  unsigned char* m[A8_TENSORS];
+  unsigned char* r[A8_TENSORS];
+  float* m_scale[A8_TENSORS];
+  float* r_scale[A8_TENSORS];
+  long sizes[A8_TENSORS];
+  int ordinal[A8_TENSORS];           // of the tensor in the optimizer, for its random numbers
+  int chunk_prefix[A8_TENSORS + 1];  // cumulative chunks
+  int ntensors;
+};
+
+struct Adam8Args {
+  double beta1_d, beta2_d;
+  float lr, beta1, beta2, rest1, rest2;  // rest = 1 - beta, of the 64-bit beta: in 32 bits 1 - 0.999 is 1e-5 off
+  float eps, bc1_recip, bc2_root_recip, decay;
+  int mode, bias_correction;
+  unsigned seed;
+  int step;
+  // capturable: read on the device at every replay
+  const float *lr_ptr, *inv_scale, *found_inf;
+  const int* step_ptr;
+};
+
+// Multiply-xorshift mixing of 32 bits; the odd multipliers are the leading
+// fractional bits of the golden ratio and of the root of 3.
+__device__ __forceinline__ unsigned mix32(unsigned x) {
+  x ^= x >> 16;
+  x *= 0x9E3779B1u;
+  x ^= x >> 15;
+  x *= 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+
+// The largest of a block's 16 lanes, on each of them: exchanges within quads, then
+// mirrored halves and rows, which need no LDS.
+__device__ __forceinline__ float max16(float v) {
+#define A8_DPP(ctrl) \
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), ctrl, 0xF, 0xF, true)))
+  A8_DPP(0xB1);   // quad_perm 1,0,3,2
+  A8_DPP(0x4E);   // quad_perm 2,3,0,1
+  A8_DPP(0x141);  // row_half_mirror
+  A8_DPP(0x140);  // row_mirror
+#undef A8_DPP
+  return v;
+}
+
+// |y| <= 448 between neighbouring codes k step and (k + 1) step; u in (0, 1) chooses.
+template <bool ROOT>
+__device__ __forceinline__ float choose(float y, float u) {
+  float a = fabsf(y);
+  a = a > E4M3_MAX ? E4M3_MAX : a;  // the maximum itself may be one rounding over; NaN stays
+  // step = 2^(exponent - 3), not under 2^-9
+  const int step_bits = max(__float_as_int(a) & 0x7F800000, 121 << 23) - (3 << 23);
+  const float step = __int_as_float(step_bits), inv = __int_as_float((254 << 23) - step_bits);
+  const float z = a * inv, k = floorf(z);
+  const bool up = ROOT ? u * fmaf(2.f, k, 1.f) < (z - k) * (z + k) : u < z - k;
+  float n = up ? k + 1.f : k;
+  if (ROOT) n = y > 0.f && n < 1.f ? 1.f : n;
+  return copysignf(n * step, y);
+}
+
+typedef float float2v __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct Eight {
+  T a[8];
+};
+
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const T* p) {
+  Eight<T> v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Eight<T>& v) {
+  __builtin_memcpy(p, &v, sizeof(v));
+}
+
+__device__ __forceinline__ void decode8(const Eight<unsigned char>& c, float* x) {
+  int w[2];
+  __builtin_memcpy(w, &c, 8);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+    x[4 * i] = lo.x;
+    x[4 * i + 1] = lo.y;
+    x[4 * i + 2] = hi.x;
+    x[4 * i + 3] = hi.y;
+  }
+}
+
+__device__ __forceinline__ Eight<unsigned char> encode8(const float* q) {
+  int w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], w[i], true);
+  }
+  Eight<unsigned char> c;
+  __builtin_memcpy(&c, w, 8);
+  return c;
+}
+
+// Scale and codes of a lane's eight values, with its block's other 15 lanes.
+template <bool ROOT>
+__device__ __forceinline__ float encode_block(const float* x, const unsigned* bits, Eight<unsigned char>& codes) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = fabsf(x[j]);
+    top = a <= 3.402823466e38f && a > top ? a : top;  // NaN and infinity are not part of it
+  }
+  top = max16(top);
+  const float scale = fmaxf(top / E4M3_MAX, 1.17549435e-38f), inv = 1.f / scale;
+  float q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned b = ROOT ? bits[j] >> 16 : bits[j] & 0xFFFFu;
+    const float u = ((float)b + 0.5f) * (1.f / 65536.f);
+    q[j] = choose<ROOT>(x[j] * inv, u) + (x[j] - x[j]);  // NaN where x is not finite
+  }
+  codes = encode8(q);
+  return scale;
+}
+
+template <typename T, bool MASTER>
+__global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Adam8Args a) {
+  __shared__ float corrections[2];
+  if (a.found_inf && *a.found_inf != 0.f) return;
+  int step = a.step;
+  if (a.step_ptr) {
+    step = *a.step_ptr;
+    if (threadIdx.x == 0) {
+      corrections[0] = a.bias_correction ? (float)(1.0 / (1.0 - pow(a.beta1_d, (double)step))) : 1.f;
+      corrections[1] = a.bias_correction ? (float)(1.0 / sqrt(1.0 - pow(a.beta2_d, (double)step))) : 1.f;
+    }
+    __syncthreads();
+    a.bc1_recip = corrections[0];
+    a.bc2_root_recip = corrections[1];
+  }
+  if (a.lr_ptr) a.lr = *a.lr_ptr;
+  const float unscale = a.inv_scale ? *a.inv_scale : 1.f;
+
+  int t = 0;
+  {
+    int hi = meta.ntensors - 1;
+    while (t < hi) {
+      const int mid = (t + hi + 1) >> 1;
+      if (meta.chunk_prefix[mid] <= (int)blockIdx.x) t = mid; else hi = mid - 1;
+    }
+  }
+  const long n = meta.sizes[t], base = (long)((int)blockIdx.x - meta.chunk_prefix[t]) * A8_CHUNK;
+  T* gp = (T*)meta.g[t];
+  T* pp = (T*)meta.p[t];
+  float* wp = (float*)meta.master[t];
+  const unsigned key = mix32(a.seed ^ mix32((unsigned)step + mix32((unsigned)meta.ordinal[t] + 0x6A09E667u)));
+
+  // all 64 lanes of a wave stay in the loop together: a block's lanes exchange their maxima
+  for (long first = base; first < min(n, base + A8_CHUNK); first += A8_BLOCK * A8_PER_LANE) {
+    const long i = first + threadIdx.x * A8_PER_LANE;
+    const int have = (int)min(max(n - i, 0L), 8L);
+    float g[8], p[8], m[8], r[8];
+    float sm = 0.f, sr = 0.f;
+    if (have) {
+      sm = meta.m_scale[t][i / A8_SCALE_BLOCK];
+      sr = meta.r_scale[t][i / A8_SCALE_BLOCK];
+    }
+    if (have == 8) {
+      const Eight<T> vg = load8(gp + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = to_float(vg.a[j]);
+      if (MASTER) {
+        const Eight<float> vw = load8(wp + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = vw.a[j];
+      } else {
+        const Eight<T> vp = load8(pp + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = to_float(vp.a[j]);
+      }
+      decode8(load8(meta.m[t] + i), m);
+      decode8(load8(meta.r[t] + i), r);
+    } else {
+      Eight<unsigned char> cm, cr;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] = j < have ? to_float(gp[i + j]) : 0.f;
+        p[j] = j < have ? (MASTER ? wp[i + j] : to_float(pp[i + j])) : 0.f;
+        cm.a[j] = j < have ? meta.m[t][i + j] : 0;
+        cr.a[j] = j < have ? meta.r[t][i + j] : 0;
+      }
+      decode8(cm, m);
+      decode8(cr, r);
+    }
+
+    unsigned bits[8];
+    const unsigned high = (unsigned)(i >> 32) * 0x6A09E667u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bits[j] = mix32(((unsigned)i + j) * 0x9E3779B1u + key + high);
+      float gj = g[j] * unscale;
+      if (a.mode == 0) gj = fmaf(a.decay, p[j], gj);
+      m[j] = fmaf(a.beta1, m[j] * sm, a.rest1 * gj);
+      const float rj = r[j] * sr;
+      r[j] = sqrtf(fmaf(a.beta2, rj * rj, a.rest2 * gj * gj));
+      float update = (m[j] * a.bc1_recip) / fmaf(r[j], a.bc2_root_recip, a.eps);
+      if (a.mode == 1) update = fmaf(a.decay, p[j], update);
+      p[j] = fmaf(-a.lr, update, p[j]);
+      if (j >= have) m[j] = r[j] = 0.f;
+    }
+
+    Eight<unsigned char> cm, cr;
+    const float new_sm = encode_block<false>(m, bits, cm);
+    const float new_sr = encode_block<true>(r, bits, cr);
+    if (have == 8) {
+      if (MASTER) {
+        Eight<float> vw;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vw.a[j] = p[j];
+        store8(wp + i, vw);
+      }
+      Eight<T> vp;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vp.a[j] = from_float<T>(p[j]);
+      store8(pp + i, vp);
+      store8(meta.m[t] + i, cm);
+      store8(meta.r[t] + i, cr);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < have) {
+          if (MASTER) wp[i + j] = p[j];
+          pp[i + j] = from_float<T>(p[j]);
+          meta.m[t][i + j] = cm.a[j];
+          meta.r[t][i + j] = cr.a[j];
+        }
+      }
+    }
+    if (have && i % A8_SCALE_BLOCK == 0) {
+      meta.m_scale[t][i / A8_SCALE_BLOCK] = new_sm;
+      meta.r_scale[t][i / A8_SCALE_BLOCK] = new_sr;
+    }
+  }
+}
+
+Adam8Args args_of(double beta1, double beta2, double eps, long mode, long bias_correction, double decay, long seed) {
+  Adam8Args a{};
+  a.beta1_d = beta1;
+  a.beta2_d = beta2;
+  a.beta1 = (float)beta1;
+  a.beta2 = (float)beta2;
+  a.rest1 = (float)(1.0 - beta1);
+  a.rest2 = (float)(1.0 - beta2);
+  a.eps = (float)eps;
+  a.decay = (float)decay;
+  a.mode = (int)mode;
+  a.bias_correction = (int)bias_correction;
+  a.seed = (unsigned)seed;
+  return a;
+}
+
+// tensor_lists: g, p, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale(, master)
+void adam_8bit(const TensorLists& lists, const std::vector<long>& ordinals, const Adam8Args& args) {
+  TORCH_CHECK(lists.size() == 6 || lists.size() == 7, "multi_tensor_adam_8bit: 6 lists, or 7 with master weights");
+  const size_t count = lists[0].size();
+  const bool master = lists.size() == 7;
+  for (auto& l : lists) TORCH_CHECK(l.size() == count, "multi_tensor_adam_8bit: tensor list length mismatch");
+  TORCH_CHECK(ordinals.size() == count, "multi_tensor_adam_8bit: one ordinal a tensor");
+  if (!count) return;
+  const auto device = lists[0][0].device();
+  const auto type = lists[1][0].scalar_type();
+  const at::DeviceGuard guard(device);
+  auto stream = current_stream();
+  Adam8Meta meta;
+  size_t t = 0;
+  while (t < count) {
+    int nt = 0;
+    long chunks = 0;
+    while (t < count && nt < A8_TENSORS) {
+      const long n = lists[1][t].numel(), blocks = (n + A8_SCALE_BLOCK - 1) / A8_SCALE_BLOCK;
+      for (size_t d = 0; d < lists.size(); ++d) {
+        const auto& x = lists[d][t];
+        const bool scales = d == 3 || d == 5;
+        TORCH_CHECK(x.device() == device, "multi_tensor_adam_8bit: tensors on more than one device");
+        TORCH_CHECK(x.numel() == (scales ? blocks : n), "multi_tensor_adam_8bit: size mismatch within tuple");
+        TORCH_CHECK(x.is_non_overlapping_and_dense(), "multi_tensor_adam_8bit: tensor not dense/contiguous");
+        TORCH_CHECK(scales || n <= 1 || x.strides() == lists[1][t].strides(),
+                    "multi_tensor_adam_8bit: layout mismatch within tensor tuple");
+        const auto want = d <= 1 ? type : d == 2 || d == 4 ? at::kFloat8_e4m3fn : at::kFloat;
+        TORCH_CHECK(x.scalar_type() == want, "multi_tensor_adam_8bit: list ", d, " must be ", want, ", got ", x.scalar_type());
+      }
+      if (n) {
+        meta.g[nt] = lists[0][t].data_ptr();
+        meta.p[nt] = lists[1][t].data_ptr();
+        meta.m[nt] = (unsigned char*)lists[2][t].data_ptr();
+        meta.m_scale[nt] = lists[3][t].data_ptr<float>();
+        meta.r[nt] = (unsigned char*)lists[4][t].data_ptr();
+        meta.r_scale[nt] = lists[5][t].data_ptr<float>();
+        meta.master[nt] = master ? lists[6][t].data_ptr() : nullptr;
+        meta.sizes[nt] = n;
+        meta.ordinal[nt] = (int)ordinals[t];
+        meta.chunk_prefix[nt] = (int)chunks;
+        chunks += (n + A8_CHUNK - 1) / A8_CHUNK;
+        // a launch's threads are counted in 32 bits
+        TORCH_CHECK(chunks < (1L << 32) / A8_BLOCK, "multi_tensor_adam_8bit: too many elements in one launch");
+        ++nt;
+      }
+      ++t;
+    }
+    if (!nt) continue;
+    meta.chunk_prefix[nt] = (int)chunks;
+    meta.ntensors = nt;
+    APEX_DISPATCH_FLOAT_HALF_BF(type, "multi_tensor_adam_8bit", ([&] {
+      if (master) {
+        hipLaunchKernelGGL((adam_8bit_kernel<scalar_t, true>), dim3((unsigned)chunks), dim3(A8_BLOCK), 0, stream, meta, args);
+      } else {
+        hipLaunchKernelGGL((adam_8bit_kernel<scalar_t, false>), dim3((unsigned)chunks), dim3(A8_BLOCK), 0, stream, meta, args);
+      }
+    }()));
+    HIP_CHECK(hipGetLastError());
+  }
+}
+
+}  // namespace
+
+void multi_tensor_adam_8bit_cuda(TensorLists tensor_lists, std::vector<long> ordinals, double lr, double beta1,
+                                 double beta2, double eps, long step, long mode, long bias_correction,
+                                 double weight_decay, long seed) {
+  Adam8Args a = args_of(beta1, beta2, eps, mode, bias_correction, weight_decay, seed);
+  a.lr = (float)lr;
+  a.bc1_recip = bias_correction ? (float)(1.0 / (1.0 - std::pow(beta1, (double)step))) : 1.f;
+  a.bc2_root_recip = bias_correction ? (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step))) : 1.f;
+  a.step = (int)step;
+  adam_8bit(tensor_lists, ordinals, a);
+}
+
+void multi_tensor_adam_8bit_capturable_cuda(TensorLists tensor_lists, std::vector<long> ordinals, at::Tensor lr,
+                                            double beta1, double beta2, double eps, at::Tensor step, long mode,
+                                            long bias_correction, double weight_decay, long seed,
+                                            c10::optional<at::Tensor> inv_scale, c10::optional<at::Tensor> found_inf) {
+  if (tensor_lists.empty() || tensor_lists[0].empty()) return;
+  const auto device = tensor_lists[0][0].device();
+  auto value = [&](const at::Tensor& t, at::ScalarType type, const char* name) {
+    TORCH_CHECK(t.device() == device && t.numel() == 1 && t.scalar_type() == type, "multi_tensor_adam_8bit: ", name,
+                " must be one ", type, " on the params' device");
+    return t.data_ptr();
+  };
+  Adam8Args a = args_of(beta1, beta2, eps, mode, bias_correction, weight_decay, seed);
+  a.lr_ptr = (const float*)value(lr, at::kFloat, "lr");
+  a.step_ptr = (const int*)value(step, at::kInt, "step");
+  if (inv_scale) a.inv_scale = (const float*)value(*inv_scale, at::kFloat, "inv_scale");
+  if (found_inf) a.found_inf = (const float*)value(*found_inf, at::kFloat, "found_inf");
+  adam_8bit(tensor_lists, ordinals, a);
+}

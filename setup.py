@@ -48,6 +48,7 @@ ext_modules = [
             "csrc/multi_tensor_l2norm.hip",
             "csrc/multi_tensor_sgd.hip",
             "csrc/multi_tensor_adam.hip",
+            "csrc/multi_tensor_adam_8bit.hip",
             "csrc/multi_tensor_opt.hip",
             "csrc/multi_tensor_lamb.hip",
             "csrc/update_scale_hysteresis.hip",

@@ -1,0 +1,202 @@
+"""FusedAdam8bit on the CPU path: its codes, the mean of its rounding, the step against 64 bits, checkpoints, refusals."""
+
+import copy
+import math
+
+import pytest
+import torch
+
+from apex_amd.optimizers import FusedAdam8bit
+from apex_amd.optimizers.fused_adam_8bit import _decode, _encode, _mix, _random_bits
+
+TABLE = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()  # 0 ... 448
+
+
+def test_random_bits_are_even():
+    """Both halves of 2^17 consecutive elements' bits, and two steps' against each other. Counts of 256 bins of 512
+    expected: a deviation over 6 sigma (136) has odds under 1e-6 for all of them together."""
+    a, b = _random_bits(3, 10, 5, 1 << 17), _random_bits(3, 11, 5, 1 << 17)
+    for bits in (a & 0xFFFF, a >> 16, (a ^ b) & 0xFFFF, (a ^ b) >> 16, (a & 0xFFFF) ^ (a >> 16), (a[1:] ^ a[:-1]) >> 16):
+        counts = torch.bincount(bits >> 8, minlength=256)
+        assert (counts - 512).abs().max() < 136
+    assert _mix(0) == 0 and 0 < _mix(1) <= 0xFFFFFFFF
+
+
+@pytest.mark.parametrize("root", [False, True])
+def test_codes_are_neighbours(root):
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(1000, generator=g) * torch.exp(4 * torch.randn(1000, generator=g))
+    x = x.abs() if root else x
+    x[5:9] = 0
+    codes, scales = _encode(x, torch.rand(1000, generator=g), root)
+    assert codes.shape == x.shape and scales.shape == (8,)
+    for b in range(8):
+        part = x[128 * b: 128 * b + 128].double()
+        assert scales[b] == (part.abs().max().float() / 448)
+        y = (part / scales[b].double()).abs().clamp(max=448)
+        got = codes[128 * b: 128 * b + 128].double()
+        assert ((got == 0) | (torch.sign(got) == torch.sign(part))).all()
+        # a y within a rounding of a code may count as on either side of it
+        lo = TABLE[(torch.searchsorted(TABLE, y * (1 - 2.0 ** -20), right=True) - 1).clamp(min=0)]
+        hi = TABLE[torch.searchsorted(TABLE, y * (1 + 2.0 ** -20)).clamp(max=126)]
+        assert ((got.abs() >= lo) & (got.abs() <= hi)).all()
+        if root:
+            assert ((got > 0) == (part > 0)).all()
+
+
+@pytest.mark.parametrize("root", [False, True])
+def test_rounding_keeps_the_mean(root):
+    """Over u = (k + 0.5) / 65536 for every k the mean is exact to a part of 65536 of the codes' distance."""
+    u = (torch.arange(65536) + 0.5) / 65536
+    for value in (447.9, 300.0, 17.3, 1.01, 0.02, 0.0021):
+        x = torch.full((65536,), value)
+        x[::128] = 448.0  # each block's scale is 1
+        codes, _ = _encode(x, u, root)
+        got = codes.double()[torch.arange(65536) % 128 != 0]
+        power = 2 if root else 1
+        i = torch.searchsorted(TABLE, value)
+        gap = TABLE[i] ** power - TABLE[i - 1] ** power
+        # the 512 left out are evenly spread over u: they move the mean by at most one part in 128 of u's own spacing
+        mean = (got ** power).mean() if root else got.mean()
+        assert abs(mean - float(torch.tensor(value)) ** power) < gap * 2e-3
+    tiny = torch.full((128,), 1e-5)
+    tiny[0] = 448.0
+    codes, _ = _encode(tiny, torch.full((128,), 0.999), root)
+    assert (codes.float()[1:] == (2.0 ** -9 if root else 0.0)).all()
+
+
+def test_a_slow_average_moves():
+    """With beta2 = 0.995 the second moment follows a gradient that becomes ten times smaller: its root falls by 0.25% a
+    step where codes are 6% and more apart, so to nearest it would stay."""
+    p = torch.nn.Parameter(torch.zeros(4096))
+    opt = FusedAdam8bit([p], lr=0.0, betas=(0.9, 0.995))
+    v, sizes = 0.0, [1.0] * 100 + [0.1] * 400
+    for s in sizes:
+        p.grad = torch.full((4096,), s)
+        v = 0.995 * v + 0.005 * s * s
+        opt.step()
+    st = opt.state[p]
+    got = (_decode(st["exp_avg_sq"], st["exp_avg_sq_scale"]).double() ** 2).mean()
+    # elements wander by some tenths of v, each for itself: the mean of 4096 by under 1%
+    assert abs(got / v - 1) < 0.05
+
+
+def reference_step(p, g, m, r, step, lr=1e-2, betas=(0.9, 0.999), eps=1e-8, wd=0.0, l2=False, bias=True):
+    p, g = p.double(), g.double()
+    if l2:
+        g = g + wd * p
+    m = betas[0] * m.double() + (1 - betas[0]) * g
+    v = betas[1] * r.double() ** 2 + (1 - betas[1]) * g * g
+    a = m / (1 - betas[0] ** step if bias else 1)
+    b = (v / (1 - betas[1] ** step if bias else 1)).sqrt() + eps
+    return p - lr * (a / b + (0.0 if l2 else wd * p)), m, v.sqrt()
+
+
+@pytest.mark.parametrize("l2,bias,master", [(False, True, False), (True, False, False), (False, True, True)])
+def test_steps_against_64_bits(l2, bias, master):
+    g = torch.Generator().manual_seed(1)
+    dtype = torch.bfloat16 if master else torch.float32
+    shapes = [(3, 50), (1,), (128,), (0,), (129,)]
+    params = [torch.nn.Parameter(torch.randn(s, generator=g).to(dtype)) for s in shapes]
+    opt = FusedAdam8bit(params, lr=1e-2, weight_decay=0.1, adam_w_mode=not l2, bias_correction=bias, master_weights=master)
+    for step in range(1, 4):
+        old = []
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=g).to(dtype)
+            st = opt.state[p]
+            old.append([p.detach().clone(), torch.zeros(p.shape), torch.zeros(p.shape)] if not st else
+                       [st.get("master_param", p.detach()).clone()] + [_decode(st[k].view(-1), st[k + "_scale"]).view(p.shape) for k in ("exp_avg", "exp_avg_sq")])
+        opt.step()
+        for p, (w, m, r) in zip(params, old):
+            want, m, r = reference_step(w, p.grad, m, r, step, wd=0.1, l2=l2, bias=bias)
+            st = opt.state[p]
+            # fp32: under 20 half steps of a weight of 4 and a step of lr * (4 + 0.4)
+            torch.testing.assert_close(st.get("master_param", p.detach()).double(), want, rtol=0, atol=20 * 2 ** -24 * 8)
+            if master:
+                assert torch.equal(p.detach(), st["master_param"].to(dtype))
+            for x, k in ((m, "exp_avg"), (r, "exp_avg_sq")):
+                got = _decode(st[k].view(-1), st[k + "_scale"]).view(p.shape).double()
+                # the code above or below: within one distance, 1/8 of the value, or the smallest, 2^-9 of the scale
+                far = x.abs() / 8 + (st[k + "_scale"].max().double() * 2 ** -9 if p.numel() else 0)
+                assert ((got - x).abs() <= far * 1.0001).all()
+
+
+def test_not_finite_stays_where_it_is():
+    p = torch.nn.Parameter(torch.ones(300))
+    opt = FusedAdam8bit([p], lr=1e-2)
+    p.grad = torch.full((300,), 0.5)
+    p.grad[7], p.grad[200] = math.inf, math.nan
+    opt.step()
+    bad = torch.zeros(300, dtype=torch.bool)
+    bad[7] = bad[200] = True
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(torch.isnan(opt.state[p][k].float()), bad)
+        assert torch.isfinite(opt.state[p][k + "_scale"]).all()
+    assert torch.equal(torch.isfinite(p.detach()), ~bad)
+
+
+def test_layouts_and_groups():
+    """A transposed weight's elements are met in memory order; a gradient of another layout is the same gradient."""
+    g = torch.Generator().manual_seed(2)
+    w, d = torch.randn(20, 30, generator=g), torch.randn(20, 30, generator=g)
+    a, b = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.t().contiguous().t())
+    assert b.stride() == (1, 20)
+    for p in (a, b):
+        opt = FusedAdam8bit([{"params": [p], "lr": 0.1}, {"params": []}], weight_decay=0.1)
+        p.grad = d.clone() if p is a else d.t().contiguous().t()
+        opt.step()
+    torch.testing.assert_close(a.detach(), b.detach(), rtol=1e-6, atol=1e-6)
+    c = torch.nn.Parameter(w.t().contiguous().t())
+    opt2 = FusedAdam8bit([c], lr=0.1, weight_decay=0.1)
+    c.grad = d.clone()
+    opt2.step()
+    assert torch.equal(b.detach(), c.detach())
+
+
+@pytest.mark.parametrize("master", [False, True])
+def test_a_checkpoint_goes_on_bit_for_bit(master):
+    g = torch.Generator().manual_seed(3)
+    start = torch.randn(5, 77, generator=g).to(torch.bfloat16 if master else torch.float32)
+    grads = [torch.randn(5, 77, generator=g).to(start.dtype) for _ in range(4)]
+
+    def go(opt, p, gs):
+        for x in gs:
+            p.grad = x.clone()
+            opt.step()
+
+    p = torch.nn.Parameter(start.clone())
+    opt = FusedAdam8bit([p], lr=1e-2, master_weights=master, seed=9)
+    go(opt, p, grads[:2])
+    saved, q = copy.deepcopy(opt.state_dict()), torch.nn.Parameter(p.detach().clone())
+    go(opt, p, grads[2:])
+    other = FusedAdam8bit([q], lr=5.0, master_weights=master, seed=9)
+    other.load_state_dict(saved)
+    st = other.state[q]
+    assert st["exp_avg"].dtype == torch.float8_e4m3fn and st["exp_avg_scale"].dtype == torch.float32
+    assert not master or st["master_param"].dtype == torch.float32
+    go(other, q, grads[2:])
+    assert torch.equal(p.detach(), q.detach())
+    for k in st:
+        assert torch.equal(opt.state[p][k].view(torch.uint8), other.state[q][k].view(torch.uint8))
+
+
+def test_refusals():
+    p = torch.nn.Parameter(torch.zeros(3))
+    with pytest.raises(RuntimeError, match="AMSGrad"):
+        FusedAdam8bit([p], amsgrad=True)
+    with pytest.raises(ValueError, match="betas"):
+        FusedAdam8bit([p], betas=(0.9, 1.0))
+    with pytest.raises(ValueError, match="eps"):
+        FusedAdam8bit([p], eps=-1.0)
+    d = torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))
+    d.grad = torch.zeros_like(d)
+    with pytest.raises(RuntimeError, match="fp16/bf16/fp32"):
+        FusedAdam8bit([d]).step()
+    e = torch.nn.Embedding(5, 3, sparse=True)
+    e(torch.tensor([1])).sum().backward()
+    with pytest.raises(RuntimeError, match="sparse"):
+        FusedAdam8bit(e.parameters()).step()
+    s = torch.nn.Parameter(torch.zeros(4, 6)[:, :3])
+    s.grad = torch.zeros(4, 3)
+    with pytest.raises(RuntimeError, match="dense"):
+        FusedAdam8bit([s]).step()
