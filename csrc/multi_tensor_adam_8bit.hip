@@ -153,7 +153,7 @@ __device__ __forceinline__ float encode_block(const float* x, const unsigned* bi
     top = a <= 3.402823466e38f && a > top ? a : top;  // NaN and infinity are not part of it
   }
   top = max16(top);
-  const float scale = fmaxf(top / E4M3_MAX, 1.17549435e-38f), inv = 1.f / scale;
+  const float scale = fmaxf(top * (1.f / E4M3_MAX), 1.17549435e-38f), inv = 1.f / scale;
   float q[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -242,9 +242,11 @@ __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Ada
       bits[j] = mix32(((unsigned)i + j) * 0x9E3779B1u + key + high);
       float gj = g[j] * unscale;
       if (a.mode == 0) gj = fmaf(a.decay, p[j], gj);
-      m[j] = fmaf(a.beta1, m[j] * sm, a.rest1 * gj);
-      const float rj = r[j] * sr;
-      r[j] = sqrtf(fmaf(a.beta2, rj * rj, a.rest2 * gj * gj));
+      // each product and sum is rounded by itself, as elementary operations do it: a code or scale that fell to the
+      // other side would show in all that follows
+      m[j] = __fadd_rn(__fmul_rn(a.beta1, __fmul_rn(m[j], sm)), __fmul_rn(a.rest1, gj));
+      const float rj = __fmul_rn(r[j], sr);
+      r[j] = sqrtf(__fadd_rn(__fmul_rn(__fmul_rn(a.beta2, rj), rj), __fmul_rn(__fmul_rn(a.rest2, gj), gj)));
       float update = (m[j] * a.bc1_recip) / fmaf(r[j], a.bc2_root_recip, a.eps);
       if (a.mode == 1) update = fmaf(a.decay, p[j], update);
       p[j] = fmaf(-a.lr, update, p[j]);

@@ -24,9 +24,6 @@
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-
 // Rows of a tensor [.., V] whose leading dimensions come down to two.
 struct Rows {
   long inner, outer_stride, inner_stride;  // row r is at (r / inner) * outer_stride + (r % inner) * inner_stride
@@ -56,41 +53,81 @@ struct Pack {
   T a[width];
 };
 
-// 16 bytes from an address that is aligned to its element only (rows of an odd V)
+// 16 bytes at an address that is aligned to its element only (rows of an odd V),
+// past the caches: nothing here is met twice in a pass
+typedef unsigned wide __attribute__((ext_vector_type(4)));
+typedef unsigned wide_at_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned wide_at_2 __attribute__((ext_vector_type(4), aligned(2)));
+
 template <typename T>
 __device__ __forceinline__ Pack<T> load16(const T* p) {
+  wide v;
+  if constexpr (sizeof(T) == 4) v = __builtin_nontemporal_load((const wide_at_4*)p);
+  else v = __builtin_nontemporal_load((const wide_at_2*)p);
   Pack<T> r;
-  __builtin_memcpy(&r, p, 16);
+  __builtin_memcpy(&r, &v, 16);
   return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void store16(T* p, const Pack<T>& v) {
-  __builtin_memcpy(p, &v, 16);
+__device__ __forceinline__ void store16(T* p, const Pack<T>& r) {
+  wide v;
+  __builtin_memcpy(&v, &r, 16);
+  if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(v, (wide_at_4*)p);
+  else __builtin_nontemporal_store(v, (wide_at_2*)p);
 }
 
-// m = max x, s = sum exp2((x - m) c), over what has been added
+// A pack of rounded floats. bf16 goes by the hardware's conversion of pairs: the
+// library's, in integer steps, takes as many instructions as all the rest.
+template <typename T>
+__device__ __forceinline__ Pack<T> rounded(const float* f) {
+  Pack<T> r;
+#pragma unroll
+  for (int j = 0; j < Pack<T>::width; ++j) r.a[j] = from_float<T>(f[j]);
+  return r;
+}
+template <>
+__device__ __forceinline__ Pack<__hip_bfloat16> rounded<__hip_bfloat16>(const float* f) {
+  typedef float float8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+  float8 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = f[j];
+  const bf16x8 b = __builtin_convertvector(v, bf16x8);
+  Pack<__hip_bfloat16> r;
+  __builtin_memcpy(&r, &b, 16);
+  return r;
+}
+
+// log2(e) / T in two parts: in one, every term of a row's sum is off to the same
+// side, and so is the sum of an answer's hundreds of log-probabilities. Both parts
+// are over 0, so that a difference of -inf stays one.
+struct Base {
+  float hi, lo;
+  __device__ __forceinline__ float exp(float d) const { return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo)); }
+};
+
+// m = max x, s = sum exp((x - m) / T), over what has been added
 struct Running {
   float m = -INFINITY, s = 0.f;
-  __device__ __forceinline__ void raise(float top, float c) {
+  // differences are taken from 0 where all so far is -inf: exp of -inf is 0
+  __device__ __forceinline__ float origin() const { return m == -INFINITY ? 0.f : m; }
+  __device__ __forceinline__ void raise(float top, Base c) {
     if (top > m) {
-      s *= __builtin_amdgcn_exp2f((m - top) * c);  // m = -inf: s is 0 and stays so
+      s *= c.exp(m - top);
       m = top;
     }
   }
-  __device__ __forceinline__ void add(float x, float c) {
-    // an m of -inf has no differences: against 0, exp2 of -inf is 0
-    s += __builtin_amdgcn_exp2f((x - (m == -INFINITY ? 0.f : m)) * c);
-  }
-  __device__ __forceinline__ void join(float mb, float sb, float c) {
-    const float top = fmaxf(m, mb), against = top == -INFINITY ? 0.f : top;
-    s = s * __builtin_amdgcn_exp2f((m - against) * c) + sb * __builtin_amdgcn_exp2f((mb - against) * c);
-    m = top;
+  __device__ __forceinline__ void join(float mb, float sb, Base c) {
+    const float ma = m;
+    m = fmaxf(m, mb);
+    const float o = origin();
+    s = s * c.exp(ma - o) + sb * c.exp(mb - o);
   }
 };
 
 template <int BLOCK>
-__device__ __forceinline__ Running block_join(Running w, float c, float* smem) {
+__device__ __forceinline__ Running block_join(Running w, Base c, float* smem) {
 #pragma unroll
   for (int off = WAVE_SIZE / 2; off > 0; off >>= 1)
     w.join(__shfl_xor(w.m, off), __shfl_xor(w.s, off), c);
@@ -102,8 +139,35 @@ __device__ __forceinline__ Running block_join(Running w, float c, float* smem) {
   __syncthreads();
   Running all;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) all.join(smem[2 * i], smem[2 * i + 1], c);
+  for (int i = 0; i < NW; ++i) all.m = fmaxf(all.m, smem[2 * i]);
+  const float o = all.origin();
+#pragma unroll
+  for (int i = 0; i < NW; ++i) all.s = fmaf(smem[2 * i + 1], c.exp(smem[2 * i] - o), all.s);
   return all;
+}
+
+// U packs into the running maximum and sum: one rescaling for all of them
+template <typename T, int U>
+__device__ __forceinline__ void take(Running& w, const Pack<T>* v, Base c) {
+  constexpr int W = Pack<T>::width;
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < W; ++j) top = fmaxf(top, to_float(v[u].a[j]));
+  w.raise(top, c);
+  const float o = w.origin();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float part = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) part += c.exp(to_float(v[u].a[j]) - o);
+    w.s += part;
+  }
+}
+
+__device__ __forceinline__ float log_prob(float x, Running w, double inv_t, float log2s) {
+  return (float)((double)(x - w.m) * inv_t - 0.6931471805599453 * (double)log2s);
 }
 
 // A block's sum in 64 bits, in a fixed order; valid on every thread.
@@ -122,52 +186,96 @@ __device__ __forceinline__ double block_sum(double v, double* smem) {
 }
 
 // ---------------- rows: maximum, sum and log-probability ----------------
+constexpr int UNROLL = 4;  // packs of a lane that are on their way together
+
 template <typename T, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) row_stats_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
-    long rows, float c, float2* __restrict__ stats, float* __restrict__ lp_out, int* __restrict__ arrived) {
+    long rows, Base c, double inv_t, float2* __restrict__ stats, float* __restrict__ lp_out,
+    int* __restrict__ arrived) {
   __shared__ float smem[2 * (BLOCK / WAVE_SIZE)];
   constexpr int W = Pack<T>::width;
   if (arrived && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // for the kernel after this one
-  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
-  const long y = labels[row];
-  if (y == ignore || y < 0 || y >= V) {
-    if (threadIdx.x == 0) {
-      const float none = y == ignore ? 0.f : NAN;
-      lp_out[row] = none;
-      stats[row] = make_float2(none, none);
-    }
-    continue;
-  }
-  const T* x = logits + where.at(row);
-  Running w;
   const long whole = V / W;
-  for (long k = threadIdx.x; k < whole; k += BLOCK) {
-    const Pack<T> v = load16(x + k * W);
-    float top = to_float(v.a[0]);
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const long y = labels[row];
+    if (y == ignore || y < 0 || y >= V) {
+      if (threadIdx.x == 0) {
+        const float none = y == ignore ? 0.f : NAN;
+        lp_out[row] = none;
+        stats[row] = make_float2(none, none);
+      }
+      continue;
+    }
+    const T* x = logits + where.at(row);
+    Running w;
+    long k = threadIdx.x;
+    for (; k + (UNROLL - 1) * BLOCK < whole; k += UNROLL * BLOCK) {
+      Pack<T> v[UNROLL];
 #pragma unroll
-    for (int j = 1; j < W; ++j) top = fmaxf(top, to_float(v.a[j]));
-    w.raise(top, c);
+      for (int u = 0; u < UNROLL; ++u) v[u] = load16(x + (k + u * BLOCK) * W);
+      take<T, UNROLL>(w, v, c);
+    }
+    if (k < whole) {
+      Pack<T> v[UNROLL - 1];
 #pragma unroll
-    for (int j = 0; j < W; ++j) w.add(to_float(v.a[j]), c);
-  }
-  for (long i = whole * W + threadIdx.x; i < V; i += BLOCK) {
-    const float f = to_float(x[i]);
-    w.raise(f, c);
-    w.add(f, c);
-  }
-  w = block_join<BLOCK>(w, c, smem);
-  if (threadIdx.x == 0) {
-    const float l2 = log2f(w.s);
-    lp_out[row] = ((to_float(x[y]) - w.m) * c - l2) * LN2;
-    stats[row] = make_float2(w.m, l2);
-  }
-  __syncthreads();  // smem is the next row's
+      for (int u = 0; u < UNROLL - 1; ++u) v[u] = load16(x + min(k + u * BLOCK, whole - 1) * W);
+#pragma unroll
+      for (int u = 0; u < UNROLL - 1; ++u)
+        if (k + u * BLOCK < whole) take<T, 1>(w, v + u, c);
+    }
+    if (const long i = whole * W + threadIdx.x; i < V) {
+      const float f = to_float(x[i]);
+      w.raise(f, c);
+      w.s += c.exp(f - w.origin());
+    }
+    w = block_join<BLOCK>(w, c, smem);
+    if (threadIdx.x == 0) {
+      const float l2 = log2f(w.s);
+      lp_out[row] = log_prob(to_float(x[y]), w, inv_t, l2);
+      stats[row] = make_float2(w.m, l2);
+    }
+    __syncthreads();  // smem is the next row's
   }
 }
 
 // ---------------- rows: gradient ----------------
+template <typename T>
+__device__ __forceinline__ Pack<T> zeros() {
+  Pack<T> z;
+#pragma unroll
+  for (int j = 0; j < Pack<T>::width; ++j) z.a[j] = from_float<T>(0.f);
+  return z;
+}
+
+// A row's f ([v = y] - p), p = exp2((x - m) c - log2 s)
+struct Gradient {
+  float f, m, l2, c;
+  long y;
+  __device__ __forceinline__ float p(float x) const { return __builtin_amdgcn_exp2f(fmaf(x - m, c, -l2)); }
+  // pack k of the row; the label's element is written over afterwards, by the lane that has just written its pack
+  template <typename T>
+  __device__ __forceinline__ void put(const Pack<T>& v, T* g, long k) const {
+    constexpr int W = Pack<T>::width;
+    float o[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = -f * p(to_float(v.a[j]));
+    store16(g + k * W, rounded<T>(o));
+    if (const unsigned long j = y - k * W; j < W) {
+      float x = to_float(v.a[0]);
+#pragma unroll
+      for (int i = 1; i < W; ++i) x = i == (int)j ? to_float(v.a[i]) : x;
+      g[y] = from_float<T>(f * (1.f - p(x)));
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void put_one(float x, T* g, long i) const {
+    g[i] = from_float<T>(f * ((i == y ? 1.f : 0.f) - p(x)));
+  }
+};
+
 // coef[r] (with `scale` and `norm`, where given) is the gradient of row r's lp.
+// A block has one pack of each lane: grid.x goes along the row, grid.y over rows.
 template <typename T, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
@@ -175,37 +283,23 @@ __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
     const float* __restrict__ scale, long scale_stride, const float* __restrict__ norm,
     T* __restrict__ grad) {
   constexpr int W = Pack<T>::width;
-  const long whole = V / W;
-  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
-  const long y = labels[row];
-  T* g = grad + row * V;
-  if (y == ignore) {
-    Pack<T> zero;
-#pragma unroll
-    for (int j = 0; j < W; ++j) zero.a[j] = from_float<T>(0.f);
-    for (long k = threadIdx.x; k < whole; k += BLOCK) store16(g + k * W, zero);
-    for (long i = whole * W + threadIdx.x; i < V; i += BLOCK) g[i] = from_float<T>(0.f);
-    continue;
-  }
-  const T* x = logits + where.at(row);
-  const float2 st = stats[row];
-  float f = coef[row] * inv_t;
-  if (scale) f *= scale[row * scale_stride];
-  if (norm) f *= *norm;
-  for (long k = threadIdx.x; k < whole; k += BLOCK) {
-    const Pack<T> v = load16(x + k * W);
-    Pack<T> o;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(to_float(v.a[j]) - st.x, c, -st.y));
-      o.a[j] = from_float<T>(f * ((k * W + j == y ? 1.f : 0.f) - p));
+  const long whole = V / W, k = (long)blockIdx.x * BLOCK + threadIdx.x;
+  for (long row = blockIdx.y; row < rows; row += gridDim.y) {
+    const long y = labels[row];
+    T* g = grad + row * V;
+    if (y == ignore) {
+      if (k < whole) store16(g + k * W, zeros<T>());
+      else if (whole * W + (k - whole) < V) g[whole * W + (k - whole)] = from_float<T>(0.f);
+      continue;
     }
-    store16(g + k * W, o);
-  }
-  for (long i = whole * W + threadIdx.x; i < V; i += BLOCK) {
-    const float p = __builtin_amdgcn_exp2f(fmaf(to_float(x[i]) - st.x, c, -st.y));
-    g[i] = from_float<T>(f * ((i == y ? 1.f : 0.f) - p));
-  }
+    const T* x = logits + where.at(row);
+    const float2 st = stats[row];
+    float f = coef[row] * inv_t;
+    if (scale) f *= scale[row * scale_stride];
+    if (norm) f *= *norm;
+    const Gradient d{f, st.x, st.y, c, y};
+    if (k < whole) d.put(load16(x + k * W), g, k);
+    else if (const long i = whole * W + (k - whole); i < V) d.put_one(to_float(x[i]), g, i);
   }
 }
 
@@ -443,6 +537,13 @@ Rows rows_of(at::Tensor& x) {
   TORCH_CHECK(false, "token_loss: logits do not come down to rows");
 }
 
+Base base_of(double temperature) {
+  const double c = 1.4426950408889634 / temperature;
+  float hi = (float)c;
+  if (hi > c) hi = std::nextafter(hi, 0.f);
+  return {hi, std::max((float)(c - hi), 1e-30f)};
+}
+
 // a launch's threads are counted in 32 bits: further rows are taken in turns
 unsigned grid_of(long rows) { return (unsigned)std::min<long>(rows, 1 << 20); }
 
@@ -486,7 +587,7 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
     constexpr int BLOCK = 256;
     hipLaunchKernelGGL((row_stats_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
                        (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
-                       (float)(1.4426950408889634 / temperature), stats, lp, arrived);
+                       base_of(temperature), 1.0 / temperature, stats, lp, arrived);
   }()));
   HIP_CHECK(hipGetLastError());
 }
@@ -522,7 +623,9 @@ at::Tensor rows_backward(at::Tensor logits, at::Tensor labels, at::Tensor stats,
   const long step = scale && scale->numel() == rows && rows > 1 ? 1 : 0;
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
     constexpr int BLOCK = 256;
-    hipLaunchKernelGGL((row_grad_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
+    const long lanes = V / Pack<scalar_t>::width + V % Pack<scalar_t>::width;
+    const dim3 grid((lanes + BLOCK - 1) / BLOCK, std::min<long>(rows, 65535));
+    hipLaunchKernelGGL((row_grad_kernel<scalar_t, BLOCK>), grid, dim3(BLOCK), 0, current_stream(),
                        (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
                        (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature),
                        (const float2*)st, co, sc, step, no, (scalar_t*)grad.data_ptr());
