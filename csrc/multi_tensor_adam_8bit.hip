@@ -29,10 +29,14 @@
 
 namespace {
 
-constexpr int A8_BLOCK = 256;          // threads
+constexpr int A8_BLOCK = 1024;         // threads
 constexpr int A8_PER_LANE = 8;         // elements: 16 lanes have a block of 128
 constexpr int A8_SCALE_BLOCK = 128;    // elements of one scale
-constexpr int A8_CHUNK = 8192;         // elements of a workgroup
+// Elements of a workgroup: each lane has one pack and is done. Workgroups that
+// went on to a second to fourth pack took 7 to 11% longer (682M elements, bf16
+// with masters: 2188 us at 4 packs of 256 threads, 1965 us at one of 1024), for
+// nothing was on its way while they rounded.
+constexpr int A8_CHUNK = A8_BLOCK * A8_PER_LANE;
 constexpr int A8_TENSORS = 48;         // of one launch: 48 * 76 B of kernel arguments
 constexpr float E4M3_MAX = 448.f;
 
@@ -85,19 +89,38 @@ __device__ __forceinline__ float max16(float v) {
   return v;
 }
 
-// |y| <= 448 between neighbouring codes k step and (k + 1) step; u in (0, 1) chooses.
-template <bool ROOT>
-__device__ __forceinline__ float choose(float y, float u) {
-  float a = fabsf(y);
-  a = a > E4M3_MAX ? E4M3_MAX : a;  // the maximum itself may be one rounding over; NaN stays
+// A |y| <= 448 lies between two neighbouring codes; u = (b + 0.5) / 65536 chooses.
+// 448 is a code: a maximum that is one rounding over it has odds under any u.
+// fma(|y|, 0, q) is q, without the sign of a -0, and NaN where y is not finite.
+
+// The first moment: up where u < z - k, z = k + rest the value in codes. In the
+// float's bits the rest is the lower 20, and the condition that rest + 2^20 -
+// (16 b + 9) carries. Under 2^-6 codes are evenly 2^-9 apart, as they are from
+// 2^-6 to 2^-5: the value is moved there and back.
+__device__ __forceinline__ float choose_linear(float y, unsigned b) {
+  const float move = fabsf(y) < 0.015625f ? 0.015625f : 0.f;
+  const unsigned carry = ((~b & 0xFFFFu) << 4) | 7u;
+  const unsigned q = (__float_as_uint(fabsf(y) + move) + carry) & 0xFFF00000u;
+  return fmaf(fabsf(y), 0.f, copysignf(__uint_as_float(q) - move, y));
+}
+
+// The root: up where u < (z^2 - k^2) / ((k + 1)^2 - k^2), and always from 0.
+__device__ __forceinline__ float choose_root(float y, unsigned b) {
+  const float u = ((float)b + 0.5f) * (1.f / 65536.f);
   // step = 2^(exponent - 3), not under 2^-9
-  const int step_bits = max(__float_as_int(a) & 0x7F800000, 121 << 23) - (3 << 23);
+  const int step_bits = max(__float_as_int(y) & 0x7F800000, 121 << 23) - (3 << 23);
   const float step = __int_as_float(step_bits), inv = __int_as_float((254 << 23) - step_bits);
-  const float z = a * inv, k = floorf(z);
-  const bool up = ROOT ? u * fmaf(2.f, k, 1.f) < (z - k) * (z + k) : u < z - k;
-  float n = up ? k + 1.f : k;
-  if (ROOT) n = y > 0.f && n < 1.f ? 1.f : n;
-  return copysignf(n * step, y);
+  const float z = y * inv, k = floorf(z);
+  const float n = u * fmaf(2.f, k, 1.f) < (z - k) * (z + k) ? k + 1.f : k;
+  return fmaf(y, 0.f, fmaxf(n, y > 0.f ? 1.f : n) * step);
+}
+
+// sqrtf but for one operand in some thousands (its last bit), in half the
+// instructions: the hardware's root (1 ulp) and one Newton step from its residual.
+__device__ __forceinline__ float root(float v) {
+  const float r = __builtin_amdgcn_sqrtf(v);
+  const float half = 0.5f * __builtin_amdgcn_rcpf(fmaxf(r, 1e-30f));
+  return fmaf(fmaf(-r, r, v), half, r);
 }
 
 typedef float float2v __attribute__((ext_vector_type(2)));
@@ -107,6 +130,16 @@ struct Eight {
   T a[8];
 };
 
+// Eight elements at an address that is aligned to its element only (views into
+// one buffer). Stores go past the caches, for a step meets each element once; the
+// loads do not: 32 bytes of a lane are two loads, whose halves share cache lines
+// (254M fp32 elements: 630 us, with loads past the caches 666 us).
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_at_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4_at_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2_at_1 __attribute__((ext_vector_type(2), aligned(1)));
+
 template <typename T>
 __device__ __forceinline__ Eight<T> load8(const T* p) {
   Eight<T> v;
@@ -115,7 +148,20 @@ __device__ __forceinline__ Eight<T> load8(const T* p) {
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const Eight<T>& v) {
-  __builtin_memcpy(p, &v, sizeof(v));
+  if constexpr (sizeof(T) == 4) {
+    u32x4 w[2];
+    __builtin_memcpy(w, &v, 32);
+    __builtin_nontemporal_store(w[0], (u32x4_at_4*)p);
+    __builtin_nontemporal_store(w[1], (u32x4_at_4*)(p + 4));
+  } else if constexpr (sizeof(T) == 2) {
+    u32x4 w;
+    __builtin_memcpy(&w, &v, 16);
+    __builtin_nontemporal_store(w, (u32x4_at_2*)p);
+  } else {
+    u32x2 w;
+    __builtin_memcpy(&w, &v, 8);
+    __builtin_nontemporal_store(w, (u32x2_at_1*)p);
+  }
 }
 
 __device__ __forceinline__ void decode8(const Eight<unsigned char>& c, float* x) {
@@ -148,19 +194,19 @@ template <bool ROOT>
 __device__ __forceinline__ float encode_block(const float* x, const unsigned* bits, Eight<unsigned char>& codes) {
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float a = fabsf(x[j]);
-    top = a <= 3.402823466e38f && a > top ? a : top;  // NaN and infinity are not part of it
-  }
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));  // NaN is no part of it
   top = max16(top);
+  if (__any(top == INFINITY)) {  // nor is infinity: hardly ever met
+    top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fabsf(x[j]) < INFINITY ? fmaxf(top, fabsf(x[j])) : top;
+    top = max16(top);
+  }
   const float scale = fmaxf(top * (1.f / E4M3_MAX), 1.17549435e-38f), inv = 1.f / scale;
   float q[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const unsigned b = ROOT ? bits[j] >> 16 : bits[j] & 0xFFFFu;
-    const float u = ((float)b + 0.5f) * (1.f / 65536.f);
-    q[j] = choose<ROOT>(x[j] * inv, u) + (x[j] - x[j]);  // NaN where x is not finite
-  }
+  for (int j = 0; j < 8; ++j)
+    q[j] = ROOT ? choose_root(x[j] * inv, bits[j] >> 16) : choose_linear(x[j] * inv, bits[j] & 0xFFFFu);
   codes = encode8(q);
   return scale;
 }
@@ -197,93 +243,110 @@ __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Ada
   float* wp = (float*)meta.master[t];
   const unsigned key = mix32(a.seed ^ mix32((unsigned)step + mix32((unsigned)meta.ordinal[t] + 0x6A09E667u)));
 
-  // all 64 lanes of a wave stay in the loop together: a block's lanes exchange their maxima
-  for (long first = base; first < min(n, base + A8_CHUNK); first += A8_BLOCK * A8_PER_LANE) {
-    const long i = first + threadIdx.x * A8_PER_LANE;
-    const int have = (int)min(max(n - i, 0L), 8L);
-    float g[8], p[8], m[8], r[8];
-    float sm = 0.f, sr = 0.f;
-    if (have) {
-      sm = meta.m_scale[t][i / A8_SCALE_BLOCK];
-      sr = meta.r_scale[t][i / A8_SCALE_BLOCK];
-    }
-    if (have == 8) {
-      const Eight<T> vg = load8(gp + i);
+  // lanes behind the tensor's end stay: a block's lanes exchange their maxima
+  const long i = base + threadIdx.x * A8_PER_LANE;
+  const int have = (int)min(max(n - i, 0L), 8L);
+  float g[8], p[8], m[8], r[8];
+  float sm = 0.f, sr = 0.f;
+  if (have) {
+    sm = meta.m_scale[t][i / A8_SCALE_BLOCK];
+    sr = meta.r_scale[t][i / A8_SCALE_BLOCK];
+  }
+  if (have == 8) {
+    const Eight<T> vg = load8(gp + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = to_float(vg.a[j]);
-      if (MASTER) {
-        const Eight<float> vw = load8(wp + i);
+    for (int j = 0; j < 8; ++j) g[j] = to_float(vg.a[j]);
+    if (MASTER) {
+      const Eight<float> vw = load8(wp + i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = vw.a[j];
-      } else {
-        const Eight<T> vp = load8(pp + i);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = to_float(vp.a[j]);
-      }
-      decode8(load8(meta.m[t] + i), m);
-      decode8(load8(meta.r[t] + i), r);
+      for (int j = 0; j < 8; ++j) p[j] = vw.a[j];
     } else {
-      Eight<unsigned char> cm, cr;
+      const Eight<T> vp = load8(pp + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        g[j] = j < have ? to_float(gp[i + j]) : 0.f;
-        p[j] = j < have ? (MASTER ? wp[i + j] : to_float(pp[i + j])) : 0.f;
-        cm.a[j] = j < have ? meta.m[t][i + j] : 0;
-        cr.a[j] = j < have ? meta.r[t][i + j] : 0;
-      }
-      decode8(cm, m);
-      decode8(cr, r);
+      for (int j = 0; j < 8; ++j) p[j] = to_float(vp.a[j]);
     }
-
-    unsigned bits[8];
-    const unsigned high = (unsigned)(i >> 32) * 0x6A09E667u;
+    decode8(load8(meta.m[t] + i), m);
+    decode8(load8(meta.r[t] + i), r);
+  } else {
+    Eight<unsigned char> cm, cr;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      bits[j] = mix32(((unsigned)i + j) * 0x9E3779B1u + key + high);
-      float gj = g[j] * unscale;
-      if (a.mode == 0) gj = fmaf(a.decay, p[j], gj);
-      // each product and sum is rounded by itself, as elementary operations do it: a code or scale that fell to the
-      // other side would show in all that follows
-      m[j] = __fadd_rn(__fmul_rn(a.beta1, __fmul_rn(m[j], sm)), __fmul_rn(a.rest1, gj));
-      const float rj = __fmul_rn(r[j], sr);
-      r[j] = sqrtf(__fadd_rn(__fmul_rn(__fmul_rn(a.beta2, rj), rj), __fmul_rn(__fmul_rn(a.rest2, gj), gj)));
-      float update = (m[j] * a.bc1_recip) / fmaf(r[j], a.bc2_root_recip, a.eps);
-      if (a.mode == 1) update = fmaf(a.decay, p[j], update);
-      p[j] = fmaf(-a.lr, update, p[j]);
-      if (j >= have) m[j] = r[j] = 0.f;
+      g[j] = j < have ? to_float(gp[i + j]) : 0.f;
+      p[j] = j < have ? (MASTER ? wp[i + j] : to_float(pp[i + j])) : 0.f;
+      cm.a[j] = j < have ? meta.m[t][i + j] : 0;
+      cr.a[j] = j < have ? meta.r[t][i + j] : 0;
     }
+    decode8(cm, m);
+    decode8(cr, r);
+  }
 
-    Eight<unsigned char> cm, cr;
-    const float new_sm = encode_block<false>(m, bits, cm);
-    const float new_sr = encode_block<true>(r, bits, cr);
-    if (have == 8) {
-      if (MASTER) {
-        Eight<float> vw;
+  if (a.inv_scale) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vw.a[j] = p[j];
-        store8(wp + i, vw);
-      }
-      Eight<T> vp;
+    for (int j = 0; j < 8; ++j) g[j] *= unscale;
+  }
+  if (a.mode == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vp.a[j] = from_float<T>(p[j]);
-      store8(pp + i, vp);
-      store8(meta.m[t] + i, cm);
-      store8(meta.r[t] + i, cr);
-    } else {
+    for (int j = 0; j < 8; ++j) g[j] = fmaf(a.decay, p[j], g[j]);
+  }
+  unsigned bits[8];
+  float update[8];
+  const unsigned high = (unsigned)(i >> 32) * 0x6A09E667u;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j < have) {
-          if (MASTER) wp[i + j] = p[j];
-          pp[i + j] = from_float<T>(p[j]);
-          meta.m[t][i + j] = cm.a[j];
-          meta.r[t][i + j] = cr.a[j];
-        }
+  for (int j = 0; j < 8; ++j) {
+    bits[j] = mix32(((unsigned)i + j) * 0x9E3779B1u + key + high);
+    // each product and sum is rounded by itself, as elementary operations do it: a code or scale that fell to the
+    // other side would show in all that follows
+    m[j] = __fadd_rn(__fmul_rn(a.beta1, __fmul_rn(m[j], sm)), __fmul_rn(a.rest1, g[j]));
+    const float rj = __fmul_rn(r[j], sr);
+    r[j] = root(__fadd_rn(__fmul_rn(__fmul_rn(a.beta2, rj), rj), __fmul_rn(__fmul_rn(a.rest2, g[j]), g[j])));
+    update[j] = (m[j] * a.bc1_recip) * __builtin_amdgcn_rcpf(fmaf(r[j], a.bc2_root_recip, a.eps));
+  }
+  if (a.mode == 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) update[j] = fmaf(a.decay, p[j], update[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    p[j] = fmaf(-a.lr, update[j], p[j]);
+    // the param is the stored master's rounding: not that of an fma that rounds to fp16 at once
+    if (MASTER) asm volatile("" : "+v"(p[j]));
+  }
+  if (have != 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j >= have) m[j] = r[j] = 0.f;
+  }
+
+  Eight<unsigned char> cm, cr;
+  const float new_sm = encode_block<false>(m, bits, cm);
+  const float new_sr = encode_block<true>(r, bits, cr);
+  if (have == 8) {
+    if (MASTER) {
+      Eight<float> vw;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vw.a[j] = p[j];
+      store8(wp + i, vw);
+    }
+    Eight<T> vp;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vp.a[j] = from_float<T>(p[j]);
+    store8(pp + i, vp);
+    store8(meta.m[t] + i, cm);
+    store8(meta.r[t] + i, cr);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < have) {
+        if (MASTER) wp[i + j] = p[j];
+        pp[i + j] = from_float<T>(p[j]);
+        meta.m[t][i + j] = cm.a[j];
+        meta.r[t][i + j] = cr.a[j];
       }
     }
-    if (have && i % A8_SCALE_BLOCK == 0) {
-      meta.m_scale[t][i / A8_SCALE_BLOCK] = new_sm;
-      meta.r_scale[t][i / A8_SCALE_BLOCK] = new_sr;
-    }
+  }
+  if (have && i % A8_SCALE_BLOCK == 0) {
+    meta.m_scale[t][i / A8_SCALE_BLOCK] = new_sm;
+    meta.r_scale[t][i / A8_SCALE_BLOCK] = new_sr;
   }
 }
 
