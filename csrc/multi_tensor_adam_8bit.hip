@@ -29,14 +29,16 @@
 
 namespace {
 
-constexpr int A8_BLOCK = 1024;         // threads
-constexpr int A8_PER_LANE = 8;         // elements: 16 lanes have a block of 128
+// Each lane has four neighbouring elements and is done: every load and store of a
+// wave is one piece without gaps, whatever the type, and may go past the caches.
+// With eight a lane (two loads of 16 bytes, 32 apart, for fp32) 682M bf16 weights
+// with masters took 2025 us and 254M fp32 weights 634 us, with four 1942 and
+// 587; with 1024 threads 2051 and 631; workgroups that went on to a second to
+// eighth part took 5 to 15% longer, for nothing was on its way while they rounded.
+constexpr int A8_BLOCK = 256;          // threads
+constexpr int A8_PER_LANE = 4;         // elements: 32 lanes have a block of 128
 constexpr int A8_SCALE_BLOCK = 128;    // elements of one scale
-// Elements of a workgroup: each lane has one pack and is done. Workgroups that
-// went on to a second to fourth pack took 7 to 11% longer (682M elements, bf16
-// with masters: 2188 us at 4 packs of 256 threads, 1965 us at one of 1024), for
-// nothing was on its way while they rounded.
-constexpr int A8_CHUNK = A8_BLOCK * A8_PER_LANE;
+constexpr int A8_CHUNK = A8_BLOCK * A8_PER_LANE;  // elements of a workgroup
 constexpr int A8_TENSORS = 48;         // of one launch: 48 * 76 B of kernel arguments
 constexpr float E4M3_MAX = 448.f;
 
@@ -76,9 +78,9 @@ __device__ __forceinline__ unsigned mix32(unsigned x) {
   return x ^ (x >> 16);
 }
 
-// The largest of a block's 16 lanes, on each of them: exchanges within quads, then
-// mirrored halves and rows, which need no LDS.
-__device__ __forceinline__ float max16(float v) {
+// The largest of a block's 32 lanes, on each of them: exchanges within quads,
+// mirrored halves and rows of 16, then between two rows. None needs LDS.
+__device__ __forceinline__ float max32(float v) {
 #define A8_DPP(ctrl) \
   v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), ctrl, 0xF, 0xF, true)))
   A8_DPP(0xB1);   // quad_perm 1,0,3,2
@@ -86,7 +88,8 @@ __device__ __forceinline__ float max16(float v) {
   A8_DPP(0x141);  // row_half_mirror
   A8_DPP(0x140);  // row_mirror
 #undef A8_DPP
-  return v;
+  const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return fmaxf(__int_as_float(rows[0]), __int_as_float(rows[1]));
 }
 
 // A |y| <= 448 lies between two neighbouring codes; u = (b + 0.5) / 65536 chooses.
@@ -126,88 +129,88 @@ __device__ __forceinline__ float root(float v) {
 typedef float float2v __attribute__((ext_vector_type(2)));
 
 template <typename T>
-struct Eight {
-  T a[8];
+struct Four {
+  T a[4];
 };
 
-// Eight elements at an address that is aligned to its element only (views into
-// one buffer). Stores go past the caches, for a step meets each element once; the
-// loads do not: 32 bytes of a lane are two loads, whose halves share cache lines
-// (254M fp32 elements: 630 us, with loads past the caches 666 us).
+// Four elements at an address that is aligned to its element only (views into one
+// buffer), past the caches: a step meets each once.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_at_4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned u32x4_at_2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x2_at_1 __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned u32x2_at_2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned u32_at_1 __attribute__((aligned(1)));
 
 template <typename T>
-__device__ __forceinline__ Eight<T> load8(const T* p) {
-  Eight<T> v;
-  __builtin_memcpy(&v, p, sizeof(v));
+__device__ __forceinline__ Four<T> load4(const T* p) {
+  Four<T> v;
+  if constexpr (sizeof(T) == 4) {
+    const u32x4 w = __builtin_nontemporal_load((const u32x4_at_4*)p);
+    __builtin_memcpy(&v, &w, 16);
+  } else if constexpr (sizeof(T) == 2) {
+    const u32x2 w = __builtin_nontemporal_load((const u32x2_at_2*)p);
+    __builtin_memcpy(&v, &w, 8);
+  } else {
+    const unsigned w = __builtin_nontemporal_load((const u32_at_1*)p);
+    __builtin_memcpy(&v, &w, 4);
+  }
   return v;
 }
+
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const Eight<T>& v) {
+__device__ __forceinline__ void store4(T* p, const Four<T>& v) {
   if constexpr (sizeof(T) == 4) {
-    u32x4 w[2];
-    __builtin_memcpy(w, &v, 32);
-    __builtin_nontemporal_store(w[0], (u32x4_at_4*)p);
-    __builtin_nontemporal_store(w[1], (u32x4_at_4*)(p + 4));
-  } else if constexpr (sizeof(T) == 2) {
     u32x4 w;
     __builtin_memcpy(&w, &v, 16);
-    __builtin_nontemporal_store(w, (u32x4_at_2*)p);
-  } else {
+    __builtin_nontemporal_store(w, (u32x4_at_4*)p);
+  } else if constexpr (sizeof(T) == 2) {
     u32x2 w;
     __builtin_memcpy(&w, &v, 8);
-    __builtin_nontemporal_store(w, (u32x2_at_1*)p);
+    __builtin_nontemporal_store(w, (u32x2_at_2*)p);
+  } else {
+    unsigned w;
+    __builtin_memcpy(&w, &v, 4);
+    __builtin_nontemporal_store(w, (u32_at_1*)p);
   }
 }
 
-__device__ __forceinline__ void decode8(const Eight<unsigned char>& c, float* x) {
-  int w[2];
-  __builtin_memcpy(w, &c, 8);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
-    x[4 * i] = lo.x;
-    x[4 * i + 1] = lo.y;
-    x[4 * i + 2] = hi.x;
-    x[4 * i + 3] = hi.y;
-  }
+__device__ __forceinline__ void decode4(const Four<unsigned char>& c, float* x) {
+  int w;
+  __builtin_memcpy(&w, &c, 4);
+  const float2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  x[0] = lo.x;
+  x[1] = lo.y;
+  x[2] = hi.x;
+  x[3] = hi.y;
 }
 
-__device__ __forceinline__ Eight<unsigned char> encode8(const float* q) {
-  int w[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
-    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], w[i], true);
-  }
-  Eight<unsigned char> c;
-  __builtin_memcpy(&c, w, 8);
+__device__ __forceinline__ Four<unsigned char> encode4(const float* q) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+  Four<unsigned char> c;
+  __builtin_memcpy(&c, &w, 4);
   return c;
 }
 
-// Scale and codes of a lane's eight values, with its block's other 15 lanes.
+// Scale and codes of a lane's four values, with its block's other 31 lanes.
 template <bool ROOT>
-__device__ __forceinline__ float encode_block(const float* x, const unsigned* bits, Eight<unsigned char>& codes) {
+__device__ __forceinline__ float encode_block(const float* x, const unsigned* bits, Four<unsigned char>& codes) {
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));  // NaN is no part of it
-  top = max16(top);
+  for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[j]));  // NaN is no part of it
+  top = max32(top);
   if (__any(top == INFINITY)) {  // nor is infinity: hardly ever met
     top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = fabsf(x[j]) < INFINITY ? fmaxf(top, fabsf(x[j])) : top;
-    top = max16(top);
+    for (int j = 0; j < 4; ++j) top = fabsf(x[j]) < INFINITY ? fmaxf(top, fabsf(x[j])) : top;
+    top = max32(top);
   }
   const float scale = fmaxf(top * (1.f / E4M3_MAX), 1.17549435e-38f), inv = 1.f / scale;
-  float q[8];
+  float q[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 4; ++j)
     q[j] = ROOT ? choose_root(x[j] * inv, bits[j] >> 16) : choose_linear(x[j] * inv, bits[j] & 0xFFFFu);
-  codes = encode8(q);
+  codes = encode4(q);
   return scale;
 }
 
@@ -245,54 +248,54 @@ __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Ada
 
   // lanes behind the tensor's end stay: a block's lanes exchange their maxima
   const long i = base + threadIdx.x * A8_PER_LANE;
-  const int have = (int)min(max(n - i, 0L), 8L);
-  float g[8], p[8], m[8], r[8];
+  const int have = (int)min(max(n - i, 0L), 4L);
+  float g[4], p[4], m[4], r[4];
   float sm = 0.f, sr = 0.f;
   if (have) {
     sm = meta.m_scale[t][i / A8_SCALE_BLOCK];
     sr = meta.r_scale[t][i / A8_SCALE_BLOCK];
   }
-  if (have == 8) {
-    const Eight<T> vg = load8(gp + i);
+  if (have == 4) {
+    const Four<T> vg = load4(gp + i);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = to_float(vg.a[j]);
+    for (int j = 0; j < 4; ++j) g[j] = to_float(vg.a[j]);
     if (MASTER) {
-      const Eight<float> vw = load8(wp + i);
+      const Four<float> vw = load4(wp + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = vw.a[j];
+      for (int j = 0; j < 4; ++j) p[j] = vw.a[j];
     } else {
-      const Eight<T> vp = load8(pp + i);
+      const Four<T> vp = load4(pp + i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = to_float(vp.a[j]);
+      for (int j = 0; j < 4; ++j) p[j] = to_float(vp.a[j]);
     }
-    decode8(load8(meta.m[t] + i), m);
-    decode8(load8(meta.r[t] + i), r);
+    decode4(load4(meta.m[t] + i), m);
+    decode4(load4(meta.r[t] + i), r);
   } else {
-    Eight<unsigned char> cm, cr;
+    Four<unsigned char> cm, cr;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 4; ++j) {
       g[j] = j < have ? to_float(gp[i + j]) : 0.f;
       p[j] = j < have ? (MASTER ? wp[i + j] : to_float(pp[i + j])) : 0.f;
       cm.a[j] = j < have ? meta.m[t][i + j] : 0;
       cr.a[j] = j < have ? meta.r[t][i + j] : 0;
     }
-    decode8(cm, m);
-    decode8(cr, r);
+    decode4(cm, m);
+    decode4(cr, r);
   }
 
   if (a.inv_scale) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] *= unscale;
+    for (int j = 0; j < 4; ++j) g[j] *= unscale;
   }
   if (a.mode == 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = fmaf(a.decay, p[j], g[j]);
+    for (int j = 0; j < 4; ++j) g[j] = fmaf(a.decay, p[j], g[j]);
   }
-  unsigned bits[8];
-  float update[8];
+  unsigned bits[4];
+  float update[4];
   const unsigned high = (unsigned)(i >> 32) * 0x6A09E667u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     bits[j] = mix32(((unsigned)i + j) * 0x9E3779B1u + key + high);
     // each product and sum is rounded by itself, as elementary operations do it: a code or scale that fell to the
     // other side would show in all that follows
@@ -303,39 +306,39 @@ __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Ada
   }
   if (a.mode == 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) update[j] = fmaf(a.decay, p[j], update[j]);
+    for (int j = 0; j < 4; ++j) update[j] = fmaf(a.decay, p[j], update[j]);
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     p[j] = fmaf(-a.lr, update[j], p[j]);
     // the param is the stored master's rounding: not that of an fma that rounds to fp16 at once
     if (MASTER) asm volatile("" : "+v"(p[j]));
   }
-  if (have != 8) {
+  if (have != 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 4; ++j)
       if (j >= have) m[j] = r[j] = 0.f;
   }
 
-  Eight<unsigned char> cm, cr;
+  Four<unsigned char> cm, cr;
   const float new_sm = encode_block<false>(m, bits, cm);
   const float new_sr = encode_block<true>(r, bits, cr);
-  if (have == 8) {
+  if (have == 4) {
     if (MASTER) {
-      Eight<float> vw;
+      Four<float> vw;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vw.a[j] = p[j];
-      store8(wp + i, vw);
+      for (int j = 0; j < 4; ++j) vw.a[j] = p[j];
+      store4(wp + i, vw);
     }
-    Eight<T> vp;
+    Four<T> vp;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vp.a[j] = from_float<T>(p[j]);
-    store8(pp + i, vp);
-    store8(meta.m[t] + i, cm);
-    store8(meta.r[t] + i, cr);
+    for (int j = 0; j < 4; ++j) vp.a[j] = from_float<T>(p[j]);
+    store4(pp + i, vp);
+    store4(meta.m[t] + i, cm);
+    store4(meta.r[t] + i, cr);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 4; ++j) {
       if (j < have) {
         if (MASTER) wp[i + j] = p[j];
         pp[i + j] = from_float<T>(p[j]);
