@@ -47,6 +47,19 @@ struct Sequences {
   }
 };
 
+// The sequence of a row, -1 where none has it
+__device__ __forceinline__ long owner_of(const Sequences& seqs, long count, long row) {
+  if (!seqs.cu) return row / seqs.length;
+  long lo = 0, hi = count - 1;  // the last one that begins at or before the row
+  while (lo < hi) {
+    const long mid = (lo + hi + 1) >> 1;
+    if (seqs.cu[mid] <= row) lo = mid; else hi = mid - 1;
+  }
+  long begin, end;
+  seqs.span(lo, begin, end);
+  return row >= begin && row < end ? lo : -1;
+}
+
 template <typename T>
 struct Pack {
   static constexpr int width = 16 / sizeof(T);
@@ -60,13 +73,21 @@ typedef unsigned wide_at_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned wide_at_2 __attribute__((ext_vector_type(4), aligned(2)));
 
 template <typename T>
-__device__ __forceinline__ Pack<T> load16(const T* p) {
-  wide v;
-  if constexpr (sizeof(T) == 4) v = __builtin_nontemporal_load((const wide_at_4*)p);
-  else v = __builtin_nontemporal_load((const wide_at_2*)p);
+__device__ __forceinline__ wide load_wide(const T* p) {
+  if constexpr (sizeof(T) == 4) return __builtin_nontemporal_load((const wide_at_4*)p);
+  else return __builtin_nontemporal_load((const wide_at_2*)p);
+}
+
+template <typename T>
+__device__ __forceinline__ Pack<T> pack_of(wide v) {
   Pack<T> r;
   __builtin_memcpy(&r, &v, 16);
   return r;
+}
+
+template <typename T>
+__device__ __forceinline__ Pack<T> load16(const T* p) {
+  return pack_of<T>(load_wide(p));
 }
 
 template <typename T>
@@ -251,31 +272,24 @@ __device__ __forceinline__ Pack<T> zeros() {
 // A row's f ([v = y] - p), p = exp2((x - m) c - log2 s)
 struct Gradient {
   float f, m, l2, c;
-  long y;
   __device__ __forceinline__ float p(float x) const { return __builtin_amdgcn_exp2f(fmaf(x - m, c, -l2)); }
-  // pack k of the row; the label's element is written over afterwards, by the lane that has just written its pack
+  __device__ __forceinline__ float at_label(float x) const { return f * (1.f - p(x)); }
+  // a pack as if it had no label
   template <typename T>
-  __device__ __forceinline__ void put(const Pack<T>& v, T* g, long k) const {
+  __device__ __forceinline__ void put(const Pack<T>& v, T* g) const {
     constexpr int W = Pack<T>::width;
     float o[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) o[j] = -f * p(to_float(v.a[j]));
-    store16(g + k * W, rounded<T>(o));
-    if (const unsigned long j = y - k * W; j < W) {
-      float x = to_float(v.a[0]);
-#pragma unroll
-      for (int i = 1; i < W; ++i) x = i == (int)j ? to_float(v.a[i]) : x;
-      g[y] = from_float<T>(f * (1.f - p(x)));
-    }
-  }
-  template <typename T>
-  __device__ __forceinline__ void put_one(float x, T* g, long i) const {
-    g[i] = from_float<T>(f * ((i == y ? 1.f : 0.f) - p(x)));
+    store16(g, rounded<T>(o));
   }
 };
 
 // coef[r] (with `scale` and `norm`, where given) is the gradient of row r's lp.
 // A block has one pack of each lane: grid.x goes along the row, grid.y over rows.
+// Blocks that take more of a row, or all of it, are slower (32768 x 50304 bf16:
+// 831 us; four packs 953, a row 995), with loads and stores through the caches
+// 905 and 1005.
 template <typename T, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
@@ -284,22 +298,26 @@ __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
     T* __restrict__ grad) {
   constexpr int W = Pack<T>::width;
   const long whole = V / W, k = (long)blockIdx.x * BLOCK + threadIdx.x;
+  // lanes behind the row's last pack have the elements that make no pack, one each
+  const long i = k < whole ? k * W : whole * W + (k - whole);
   for (long row = blockIdx.y; row < rows; row += gridDim.y) {
     const long y = labels[row];
     T* g = grad + row * V;
-    if (y == ignore) {
-      if (k < whole) store16(g + k * W, zeros<T>());
-      else if (whole * W + (k - whole) < V) g[whole * W + (k - whole)] = from_float<T>(0.f);
+    float f = coef[row] * inv_t;
+    if (scale) f *= scale[row * scale_stride];
+    if (norm) f *= *norm;
+    if (y == ignore || f == 0.f) {  // a clipped token, or one that no sequence has: its logits are not asked
+      if (k < whole) store16(g + i, zeros<T>());
+      else if (i < V) g[i] = from_float<T>(0.f);
       continue;
     }
     const T* x = logits + where.at(row);
     const float2 st = stats[row];
-    float f = coef[row] * inv_t;
-    if (scale) f *= scale[row * scale_stride];
-    if (norm) f *= *norm;
-    const Gradient d{f, st.x, st.y, c, y};
-    if (k < whole) d.put(load16(x + k * W), g, k);
-    else if (const long i = whole * W + (k - whole); i < V) d.put_one(to_float(x[i]), g, i);
+    const Gradient d{f, st.x, st.y, c};
+    if (k < whole) d.put(load16(x + i), g + i);
+    else if (i < V) g[i] = from_float<T>(-f * d.p(to_float(x[i])));
+    // the label's element, by the lane that has just written its pack
+    if (y >= 0 && y < V && (k < whole ? y >= i && y < i + W : y == i)) g[y] = from_float<T>(d.at_label(to_float(x[y])));
   }
 }
 
@@ -492,9 +510,126 @@ __global__ void __launch_bounds__(SEQ_BLOCK) policy_kernel(
   }
 }
 
-// What the gradient is multiplied by, of a number and a value on the device.
-__global__ void scale_kernel(float number, const float* __restrict__ value, float* __restrict__ applied) {
-  *applied = value ? number * *value : number;
+// ---------------- policy loss and gradient at once ----------------
+// Where the gradient of the loss is known beforehand, a row's logits are read
+// once: a block holds them in registers from the first use to the second.
+
+// What has to be known before: the weight of a token in the loss (of each
+// sequence, or weights[0] for all), and what the gradient is multiplied by.
+constexpr int PREPARE_BLOCK = 1024;
+__global__ void __launch_bounds__(PREPARE_BLOCK) policy_prepare_kernel(
+    const long* __restrict__ labels, long ignore, Sequences seqs, long count, int reduction, float number,
+    const float* __restrict__ value, float* __restrict__ applied, float* __restrict__ weights,
+    int* __restrict__ arrived) {
+  __shared__ double smem[PREPARE_BLOCK / WAVE_SIZE];
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *applied = value ? number * *value : number;
+    *arrived = 0;
+  }
+  long begin, end, unused;
+  seqs.span(reduction == SEQUENCE ? blockIdx.x : 0, begin, end);
+  if (reduction != SEQUENCE) seqs.span(count - 1, unused, end);
+  int n = 0;
+  if (reduction != SUM) {
+#pragma unroll 4
+    for (long r = begin + threadIdx.x; r < end; r += PREPARE_BLOCK) n += labels[r] != ignore ? 1 : 0;
+  }
+  const double all = block_sum<PREPARE_BLOCK>((double)n, smem);
+  if (threadIdx.x == 0)
+    weights[blockIdx.x] = (float)(reduction == SUM ? 1.0 : 1.0 / (fmax(all, 1.0) * (reduction == SEQUENCE ? (double)count : 1.0)));
+}
+
+// One block a row, at most NP packs a lane and more than NP - 2: all but the last
+// two are there without a question.
+template <typename T, int BLOCK, int NP>
+__global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
+    const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V, long first_row,
+    Base c, double inv_t, Sequences seqs, long count, Policy policy, bool weight_by_sequence,
+    const float* __restrict__ weights, const float* __restrict__ applied, float* __restrict__ lp_out,
+    float* __restrict__ losses, T* __restrict__ grad) {
+  __shared__ float smem[2 * (BLOCK / WAVE_SIZE)];
+  constexpr int W = Pack<T>::width;
+  const long row = first_row + blockIdx.x;
+  const long y = labels[row];
+  T* g = grad + row * V;
+  const int whole = (int)(V / W), tail = whole * W + (int)threadIdx.x, lane = threadIdx.x * W;
+  const auto put_zeros = [&] {
+    for (int k = threadIdx.x; k < whole; k += BLOCK) store16(g + k * W, zeros<T>());
+    if (tail < V) g[tail] = from_float<T>(0.f);
+  };
+  if (y == ignore) {
+    if (threadIdx.x == 0) lp_out[row] = losses[row] = 0.f;
+    put_zeros();
+    return;
+  }
+  const T* x = logits + where.at(row);
+  const bool in = y >= 0 && y < V;
+  const T xy = x[in ? y : 0];
+  const bool has[2] = {(NP - 2) * BLOCK + (int)threadIdx.x < whole, (NP - 1) * BLOCK + (int)threadIdx.x < whole};
+  wide v[NP];
+#pragma unroll
+  for (int u = 0; u < NP; ++u)
+    if (u < NP - 2 || has[u - (NP - 2)]) v[u] = load_wide(x + u * BLOCK * W + lane);
+  T xt = from_float<T>(-INFINITY);
+  if (tail < V) xt = x[tail];
+  Running w;
+#pragma unroll
+  for (int u = 0; u < NP; ++u)
+    if (u < NP - 2 || has[u - (NP - 2)]) {
+      const Pack<T> some = pack_of<T>(v[u]);
+      take<T, 1>(w, &some, c);
+      __builtin_amdgcn_sched_barrier(0);  // one pack's floats at a time: the packs take half of the registers
+    }
+  w.raise(to_float(xt), c);
+  w.s += c.exp(to_float(xt) - w.origin());
+  w = block_join<BLOCK>(w, c, smem);
+  const float l2 = log2f(w.s), lp = log_prob(in ? to_float(xy) : NAN, w, inv_t, l2);
+  float f = 0.f, loss = 0.f;
+  const long s = owner_of(seqs, count, row);
+  if (s >= 0) {
+    float slope;
+    const float weight = weights[weight_by_sequence ? s : 0];
+    loss = weight * policy.of(lp, row, s, slope);
+    f = weight * slope * *applied * (float)inv_t;
+  }
+  if (threadIdx.x == 0) {
+    lp_out[row] = lp;
+    losses[row] = loss;
+  }
+  if (f == 0.f) {
+    put_zeros();
+    return;
+  }
+  const Gradient d{f, w.m, l2, c.hi};
+#pragma unroll
+  for (int u = 0; u < NP; ++u)
+    if (u < NP - 2 || has[u - (NP - 2)]) {
+      // converted again: kept from the first use, the floats would take twice the registers
+      asm volatile("" : "+v"(v[u]));
+      d.put(pack_of<T>(v[u]), g + u * BLOCK * W + lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  if (tail < V) g[tail] = from_float<T>(-f * d.p(to_float(xt)));
+  // the label's element, by the lane that has just written its pack
+  if (in && (y < whole * W ? (y / W) % BLOCK == threadIdx.x : y == tail)) g[y] = from_float<T>(d.at_label(to_float(xy)));
+}
+
+// The rows' weighted losses, in a fixed order and 64 bits
+constexpr int TOTAL_BLOCK = 1024;
+__global__ void __launch_bounds__(TOTAL_BLOCK) total_kernel(const float* __restrict__ losses, long rows,
+                                                            double* __restrict__ partial, int* __restrict__ arrived,
+                                                            float* __restrict__ loss_out) {
+  __shared__ double smem[TOTAL_BLOCK / WAVE_SIZE];
+  __shared__ int last;
+  double sum = 0;
+  for (long r = (long)blockIdx.x * TOTAL_BLOCK + threadIdx.x; r < rows; r += (long)gridDim.x * TOTAL_BLOCK) sum += losses[r];
+  sum = block_sum<TOTAL_BLOCK>(sum, smem);
+  if (gridDim.x > 1) {
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    if (!comes_last(arrived, gridDim.x, &last)) return;
+    sum = block_sum<TOTAL_BLOCK>(threadIdx.x < gridDim.x ? read_shared(partial + threadIdx.x) : 0.0, smem);
+  }
+  if (threadIdx.x == 0) *loss_out = (float)sum;
 }
 
 // A gradient made for `applied` becomes that for *scale. Most often they are the same and nothing is moved.
@@ -577,6 +712,14 @@ Sequences sequences_of(const at::Tensor& labels, const c10::optional<at::Tensor>
     TORCH_CHECK(count > 0 && labels.numel() % count == 0, "token_loss: rows do not divide into sequences");
   }
   return s;
+}
+
+Policy policy_of(const at::Tensor& logits, const c10::optional<at::Tensor>& old, const at::Tensor& advantages,
+                 bool by_row, const c10::optional<at::Tensor>& ref, long rows, long count, double low, double high,
+                 double kl) {
+  return {old ? floats(*old, logits, rows, "old_log_probs") : nullptr,
+          ref ? floats(*ref, logits, rows, "ref_log_probs") : nullptr,
+          floats(advantages, logits, by_row ? rows : count, "advantages"), by_row, (float)low, (float)high, (float)kl};
 }
 
 void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, double temperature,
@@ -705,10 +848,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_fo
   const long rows = labels.numel();
   TORCH_CHECK(rows > 0 && count > 0, "policy_loss: needs a sequence and a row");
   const Sequences seqs = sequences_of(labels, cu, count);
-  Policy policy{old ? floats(*old, logits, rows, "old_log_probs") : nullptr,
-                ref ? floats(*ref, logits, rows, "ref_log_probs") : nullptr,
-                floats(advantages, logits, by_row ? rows : count, "advantages"), by_row, (float)low, (float)high,
-                (float)kl};
+  const Policy policy = policy_of(logits, old, advantages, by_row, ref, rows, count, low, high, kl);
   auto opts = logits.options().dtype(at::kFloat);
   auto lp = at::empty(labels.sizes(), opts);
   auto stats = at::empty({rows, 2}, opts);
@@ -736,12 +876,63 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
     double temperature, long reduction, long ignore, double scale, c10::optional<at::Tensor> scale_tensor) {
   check_rows(logits, labels);
   const at::DeviceGuard guard(logits.device());
-  auto applied = at::empty({1}, logits.options().dtype(at::kFloat));
+  const long rows = labels.numel(), V = logits.size(-1);
+  TORCH_CHECK(rows > 0 && count > 0, "policy_loss: needs a sequence and a row");
+  TORCH_CHECK(reduction != NONE, "policy_loss: a gradient at once needs a loss of one number");
+  auto opts = logits.options().dtype(at::kFloat);
+  const Sequences seqs = sequences_of(labels, cu, count);
+  const Policy policy = policy_of(logits, old, advantages, by_row, ref, rows, count, low, high, kl);
   const float* value = scale_tensor ? floats(*scale_tensor, logits, 1, "grad_scale") : nullptr;
-  hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1), 0, current_stream(), (float)scale, value, applied.data_ptr<float>());
-  auto [loss, lp, stats, coef, norm] = policy_forward(logits, labels, old, advantages, by_row, ref, cu, count, low, high,
-                                                      kl, temperature, reduction, ignore);
-  auto grad = rows_backward(logits, labels, stats, coef, applied, norm, ignore, temperature);
+  const long groups = reduction == SEQUENCE ? count : 1;
+  auto loss = at::empty({}, opts), lp = at::empty(labels.sizes(), opts), applied = at::empty({1}, opts);
+  auto room = at::empty({groups + rows}, opts);  // weights, and the rows' losses
+  auto partial = at::empty({64 + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
+  int* arrived = (int*)(partial.data_ptr<double>() + 64);
+  float *weights = room.data_ptr<float>(), *losses = weights + groups;
+  hipLaunchKernelGGL(policy_prepare_kernel, dim3(groups), dim3(PREPARE_BLOCK), 0, current_stream(),
+                     labels.data_ptr<long>(), ignore, seqs, count, (int)reduction, (float)scale, value,
+                     applied.data_ptr<float>(), weights, arrived);
+  HIP_CHECK(hipGetLastError());
+  at::Tensor grad;
+  bool held = false;
+  APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "policy_loss", ([&] {
+    const long whole = V / Pack<scalar_t>::width;
+    auto launch = [&](auto block, auto packs) {
+      constexpr int BLOCK = decltype(block)::value, NP = decltype(packs)::value;
+      if (held || whole > BLOCK * NP) return;
+      held = true;
+      grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+      const Rows where = rows_of(logits);
+      constexpr long MOST = 1 << 20;  // a launch's threads are counted in 32 bits
+      for (long first = 0; first < rows; first += MOST)
+        hipLaunchKernelGGL((policy_at_once_kernel<scalar_t, BLOCK, NP>), dim3(std::min(MOST, rows - first)),
+                           dim3(BLOCK), 0, current_stream(), (const scalar_t*)logits.data_ptr(), where,
+                           labels.data_ptr<long>(), ignore, V, first, base_of(temperature), 1.0 / temperature, seqs,
+                           count, policy, reduction == SEQUENCE, weights, applied.data_ptr<float>(),
+                           lp.data_ptr<float>(), losses, (scalar_t*)grad.data_ptr());
+    };
+    auto launch_of = [&](auto block, auto... packs) { (launch(block, packs), ...); };
+    // the fewest lanes that hold a row in up to 16 packs each: there is room for other rows on the compute unit then,
+    // which read while this one waits for its sum
+    using std::integral_constant;
+    launch_of(integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{},
+              integral_constant<int, 6>{}, integral_constant<int, 8>{}, integral_constant<int, 10>{},
+              integral_constant<int, 12>{}, integral_constant<int, 14>{}, integral_constant<int, 16>{});
+    launch_of(integral_constant<int, 512>{}, integral_constant<int, 10>{}, integral_constant<int, 12>{},
+              integral_constant<int, 14>{}, integral_constant<int, 16>{});
+    launch_of(integral_constant<int, 1024>{}, integral_constant<int, 10>{}, integral_constant<int, 12>{},
+              integral_constant<int, 14>{}, integral_constant<int, 16>{});
+  }()));
+  HIP_CHECK(hipGetLastError());
+  if (!held) {  // a longer row is read twice
+    auto [loss2, lp2, stats, coef, norm] = policy_forward(logits, labels, old, advantages, by_row, ref, cu, count, low,
+                                                          high, kl, temperature, reduction, ignore);
+    return {loss2, lp2, rows_backward(logits, labels, stats, coef, applied, norm, ignore, temperature), applied};
+  }
+  const long blocks = std::min<long>(64, (rows + 4 * TOTAL_BLOCK - 1) / (4 * TOTAL_BLOCK));
+  hipLaunchKernelGGL(total_kernel, dim3(blocks), dim3(TOTAL_BLOCK), 0, current_stream(), losses, rows,
+                     partial.data_ptr<double>(), arrived, loss.data_ptr<float>());
+  HIP_CHECK(hipGetLastError());
   return {loss, lp, grad, applied};
 }
 
