@@ -19,7 +19,6 @@ raises. Passes can be captured into a hipGraph.
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..._ext import get_ext
 
@@ -56,6 +55,8 @@ def _check_sequences(labels, cu_seqlens):
         raise ValueError(f"with cu_seqlens labels must be 1-D, got {tuple(labels.shape)}")
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype != torch.int32:
         raise ValueError("cu_seqlens must be 1-D int32 with one value more than there are sequences")
+    if not cu_seqlens.is_contiguous():
+        raise ValueError("cu_seqlens must be contiguous")
     if cu_seqlens.device != labels.device:
         raise ValueError(f"cu_seqlens are on {cu_seqlens.device}, labels on {labels.device}")
     return cu_seqlens.numel() - 1
@@ -69,7 +70,7 @@ def _given(t, name, like, *shapes):
         raise TypeError(f"{name} must be floating point, got {t.dtype}")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, logits on {like.device}")
-    return t.detach().float().contiguous()
+    return t.detach() if t.dtype == torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
 
 
 # ---- CPU path: plain torch, differentiated by autograd ----
@@ -105,48 +106,13 @@ def _ref_sums(lp, labels, ignore_index, cu_seqlens, count, average):
 # ---- log-probabilities ----
 
 
-class TokenLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ignore_index, temperature):
-        lp, stats = get_ext("token_loss").token_forward(logits, labels, ignore_index, temperature)
-        ctx.save_for_backward(logits, labels, stats)
-        ctx.args = ignore_index, temperature
-        return lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, labels, stats = ctx.saved_tensors
-        dlogits = get_ext("token_loss").rows_backward(logits, labels, stats, grad.float().contiguous(), None, None, *ctx.args)
-        return dlogits, None, None, None
-
-
 def token_log_probs(logits, labels, ignore_index=-100, temperature=1.0):
     """Log-probability of each label under ``softmax(logits / temperature)``: fp32, of the labels' shape, 0 where the
     label is ``ignore_index``. Differentiable in the logits."""
     labels = _check(logits, labels, ignore_index, temperature)
     if logits.is_cuda:
-        return TokenLogProbs.apply(logits, labels, ignore_index, float(temperature))
+        return get_ext("token_loss").token_log_probs(logits, labels, ignore_index, temperature)
     return _ref_log_probs(logits, labels, ignore_index, temperature)
-
-
-class SequenceLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, cu_seqlens, count, average, ignore_index, temperature):
-        sums, stats = get_ext("token_loss").sequence_forward(logits, labels, cu_seqlens, count, average, ignore_index, temperature)
-        ctx.save_for_backward(logits, labels, stats, cu_seqlens)
-        ctx.args = average, ignore_index, temperature
-        return sums
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, labels, stats, cu_seqlens = ctx.saved_tensors
-        average, ignore_index, temperature = ctx.args
-        ext = get_ext("token_loss")
-        coef = ext.sequence_coef(grad.float().contiguous(), labels, cu_seqlens, average, ignore_index)
-        dlogits = ext.rows_backward(logits, labels, stats, coef, None, None, ignore_index, temperature)
-        return dlogits, None, None, None, None, None, None
 
 
 def sequence_log_probs(logits, labels, cu_seqlens=None, average=False, ignore_index=-100, temperature=1.0):
@@ -157,31 +123,12 @@ def sequence_log_probs(logits, labels, cu_seqlens=None, average=False, ignore_in
     labels = _check(logits, labels, ignore_index, temperature)
     count = _check_sequences(labels, cu_seqlens)
     if logits.is_cuda:
-        cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
-        return SequenceLogProbs.apply(logits, labels, cu_seqlens, count, bool(average), ignore_index, float(temperature))
+        return get_ext("token_loss").sequence_log_probs(logits, labels, cu_seqlens, count, bool(average), ignore_index, temperature)
     lp = _ref_log_probs(logits, labels, ignore_index, temperature)
     return _ref_sums(lp, labels, ignore_index, cu_seqlens, count, average).float()
 
 
 # ---- paired log ratios ----
-
-
-class PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ref, cu_seqlens, pairs, kind, beta, smoothing, average, ignore_index):
-        loss, rewards, stats, coef = get_ext("token_loss").preference_forward(
-            logits, labels, ref, cu_seqlens, pairs, kind, beta, smoothing, average, ignore_index)
-        ctx.save_for_backward(logits, labels, stats, coef)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(rewards)
-        return loss, rewards
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, _):
-        logits, labels, stats, coef = ctx.saved_tensors
-        dlogits = get_ext("token_loss").rows_backward(logits, labels, stats, coef, grad.float(), None, ctx.ignore_index, 1.0)
-        return (dlogits,) + (None,) * 9
 
 
 def preference_loss(logits, labels, ref_log_probs, beta=0.1, label_smoothing=0.0, loss_type="sigmoid", average=False,
@@ -220,10 +167,8 @@ def preference_loss(logits, labels, ref_log_probs, beta=0.1, label_smoothing=0.0
     ref = _given(ref_log_probs, "ref_log_probs", logits, (count,))
     pairs = count // 2
     if logits.is_cuda:
-        cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
-        loss, rewards = PreferenceLoss.apply(logits, labels, ref, cu_seqlens, pairs, _KINDS[loss_type], float(beta),
-                                             float(label_smoothing), bool(average), ignore_index)
-        return loss, rewards[:pairs], rewards[pairs:]
+        return tuple(get_ext("token_loss").preference_loss(logits, labels, ref, cu_seqlens, pairs, _KINDS[loss_type], beta,
+                                                           label_smoothing, bool(average), ignore_index))
     lp = _ref_log_probs(logits, labels, ignore_index, 1.0)
     gain = _ref_sums(lp, labels, ignore_index, cu_seqlens, count, average) - ref.double()
     z = beta * (gain[:pairs] - gain[pairs:])
@@ -239,49 +184,6 @@ def preference_loss(logits, labels, ref_log_probs, beta=0.1, label_smoothing=0.0
 
 
 # ---- clipped policy loss ----
-
-
-class PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, old, advantages, by_row, ref, cu_seqlens, count, low, high, kl, temperature,
-                reduction, ignore_index):
-        loss, lp, stats, coef, norm = get_ext("token_loss").policy_forward(
-            logits, labels, old, advantages, by_row, ref, cu_seqlens, count, low, high, kl, temperature, reduction, ignore_index)
-        ctx.save_for_backward(logits, labels, stats, coef, norm if reduction == _REDUCTIONS["token"] else None)
-        ctx.args = ignore_index, temperature
-        ctx.mark_non_differentiable(lp)
-        return loss, lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, _):
-        logits, labels, stats, coef, norm = ctx.saved_tensors
-        dlogits = get_ext("token_loss").rows_backward(logits, labels, stats, coef, grad.float().contiguous(), norm, *ctx.args)
-        return (dlogits,) + (None,) * 13
-
-
-class PolicyLossAtOnce(torch.autograd.Function):
-    """The loss and, in the same pass over the logits, their gradient for a gradient of the loss that is known."""
-
-    @staticmethod
-    def forward(ctx, logits, labels, old, advantages, by_row, ref, cu_seqlens, count, low, high, kl, temperature,
-                reduction, ignore_index, scale, scale_tensor):
-        ext = get_ext("token_loss")
-        loss, lp, dlogits, applied = ext.policy_at_once(
-            logits, labels, old, advantages, by_row, ref, cu_seqlens, count, low, high, kl, temperature, reduction,
-            ignore_index, scale, scale_tensor)
-        ctx.made = dlogits, applied
-        ctx.mark_non_differentiable(lp)
-        return loss, lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, _):
-        if ctx.made is None:
-            raise RuntimeError("policy_loss(grad_scale=...) made its gradient in the forward pass: it can be taken once only")
-        (dlogits, applied), ctx.made = ctx.made, None
-        get_ext("token_loss").rescale_(dlogits, grad.float(), applied)
-        return (dlogits,) + (None,) * 15
 
 
 def policy_loss(logits, labels, old_log_probs, advantages, ref_log_probs=None, clip_eps=0.2, clip_eps_high=None,
@@ -341,14 +243,12 @@ def policy_loss(logits, labels, old_log_probs, advantages, ref_log_probs=None, c
                 raise ValueError("grad_scale must be a number, or one fp32 value on the logits' device")
         elif not (math.isfinite(grad_scale) and grad_scale != 0):
             raise ValueError(f"grad_scale must be finite and not 0, got {grad_scale}")
-    args = (labels, old, advantages, by_row, ref, cu_seqlens, count, float(clip_eps), float(high), float(kl_coef),
-            float(temperature), _REDUCTIONS[reduction], ignore_index)
+    args = (labels, old, advantages, by_row, ref, cu_seqlens, count, clip_eps, high, kl_coef, temperature,
+            _REDUCTIONS[reduction], ignore_index)
     if logits.is_cuda:
-        args = args[:5] + (None if cu_seqlens is None else cu_seqlens.contiguous(),) + args[6:]
-        if grad_scale is not None and logits.requires_grad and torch.is_grad_enabled():
-            tensor = grad_scale.detach().reshape(1) if torch.is_tensor(grad_scale) else None
-            return PolicyLossAtOnce.apply(logits, *args, 1.0 if tensor is not None else float(grad_scale), tensor)
-        return PolicyLoss.apply(logits, *args)
+        tensor = grad_scale.detach().reshape(1) if torch.is_tensor(grad_scale) else None
+        number = 1.0 if tensor is not None or grad_scale is None else grad_scale
+        return tuple(get_ext("token_loss").policy_loss(logits, *args, grad_scale is not None, number, tensor))
     lp = _ref_log_probs(logits, labels, ignore_index, temperature)
     return _ref_policy(lp, *args)
 

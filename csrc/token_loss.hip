@@ -16,12 +16,14 @@
 #include "common.h"
 
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <cmath>
 #include <limits>
 #include <tuple>
 #include <vector>
 
+// All in one file: nothing is called from elsewhere but through the module.
 namespace {
 
 // Rows of a tensor [.., V] whose leading dimensions come down to two.
@@ -191,19 +193,25 @@ __device__ __forceinline__ float log_prob(float x, Running w, double inv_t, floa
   return (float)((double)(x - w.m) * inv_t - 0.6931471805599453 * (double)log2s);
 }
 
-// A block's sum in 64 bits, in a fixed order; valid on every thread.
-template <int BLOCK>
-__device__ __forceinline__ double block_sum(double v, double* smem) {
-#pragma unroll
-  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
+// A block's sums of N values in 64 bits, in a fixed order; valid on every thread.
+template <int BLOCK, int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double* smem /* N * waves */) {
   constexpr int NW = BLOCK / WAVE_SIZE;
-  __syncthreads();
-  if ((threadIdx.x & (WAVE_SIZE - 1)) == 0) smem[threadIdx.x / WAVE_SIZE] = v;
-  __syncthreads();
-  double all = 0;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) all += smem[i];
-  return all;
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) v[n] += __shfl_xor(v[n], off);
+  __syncthreads();  // of what was read from smem before
+  if ((threadIdx.x & (WAVE_SIZE - 1)) == 0)
+#pragma unroll
+    for (int n = 0; n < N; ++n) smem[n * NW + threadIdx.x / WAVE_SIZE] = v[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    v[n] = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v[n] += smem[n * NW + i];
+  }
 }
 
 // ---------------- rows: maximum, sum and log-probability ----------------
@@ -257,6 +265,67 @@ __global__ void __launch_bounds__(BLOCK) row_stats_kernel(
       stats[row] = make_float2(w.m, l2);
     }
     __syncthreads();  // smem is the next row's
+  }
+}
+
+// Few long rows: a block has UNROLL packs of each lane, a second kernel joins a
+// row's parts. Along grid.x are the parts of a row.
+constexpr int PART_BLOCK = 256, PART_PACKS = PART_BLOCK * UNROLL;
+
+template <typename T>
+__global__ void __launch_bounds__(PART_BLOCK) row_part_kernel(
+    const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V, Base c,
+    float2* __restrict__ parts, int* __restrict__ arrived) {
+  __shared__ float smem[2 * (PART_BLOCK / WAVE_SIZE)];
+  constexpr int W = Pack<T>::width;
+  const long row = blockIdx.y, whole = V / W;
+  if (arrived && blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0) *arrived = 0;  // for the kernel after the next
+  if (labels[row] == ignore) return;
+  const T* x = logits + where.at(row);
+  Running w;
+  const long k = (long)blockIdx.x * PART_PACKS + threadIdx.x;
+  Pack<T> v[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u)
+    if (k + u * PART_BLOCK < whole) v[u] = load16(x + (k + u * PART_BLOCK) * W);
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u)
+    if (k + u * PART_BLOCK < whole) take<T, 1>(w, v + u, c);
+  if (const long i = whole * W + threadIdx.x; blockIdx.x == gridDim.x - 1 && i < V) {
+    const float f = to_float(x[i]);
+    w.raise(f, c);
+    w.s += c.exp(f - w.origin());
+  }
+  w = block_join<PART_BLOCK>(w, c, smem);
+  if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float2(w.m, w.s);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(WAVE_SIZE) row_join_kernel(
+    const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V, Base c,
+    double inv_t, const float2* __restrict__ parts, int count, float2* __restrict__ stats,
+    float* __restrict__ lp_out) {
+  const long row = blockIdx.x, y = labels[row];
+  if (y == ignore || y < 0 || y >= V) {
+    if (threadIdx.x == 0) {
+      const float none = y == ignore ? 0.f : NAN;
+      lp_out[row] = none;
+      stats[row] = make_float2(none, none);
+    }
+    return;
+  }
+  const float xy = to_float(logits[where.at(row) + y]);
+  Running w;
+  for (int i = threadIdx.x; i < count; i += WAVE_SIZE) {
+    const float2 part = parts[row * count + i];
+    w.join(part.x, part.y, c);
+  }
+#pragma unroll
+  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) w.join(__shfl_xor(w.m, off), __shfl_xor(w.s, off), c);
+  if (threadIdx.x == 0) {
+    const float l2 = log2f(w.s);
+    lp_out[row] = log_prob(xy, w, inv_t, l2);
+    stats[row] = make_float2(w.m, l2);
   }
 }
 
@@ -322,45 +391,50 @@ __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
 }
 
 // ---------------- sequences ----------------
-constexpr int SEQ_BLOCK = 256;
+// A block has a sequence (or a pair): 256 threads, or 1024 where sequences are long.
 
-// Sum (in 64 bits) and number of a sequence's labelled lp.
+// A lane's sum (in 64 bits) and number of a sequence's labelled lp.
+template <int BLOCK>
 __device__ __forceinline__ void sum_span(const float* lp, const long* labels, long ignore, long begin,
-                                         long end, double* smem, double& sum, double& count) {
-  double s = 0, n = 0;
-  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) {
+                                         long end, double& sum, double& count) {
+  sum = count = 0;
+#pragma unroll 2
+  for (long r = begin + threadIdx.x; r < end; r += BLOCK) {
+    const float v = lp[r];
     const bool on = labels[r] != ignore;
-    s += on ? (double)lp[r] : 0.0;
-    n += on ? 1.0 : 0.0;
+    sum += on ? (double)v : 0.0;
+    count += on ? 1.0 : 0.0;
   }
-  sum = block_sum<SEQ_BLOCK>(s, smem);
-  count = block_sum<SEQ_BLOCK>(n, smem);
 }
 
-__global__ void __launch_bounds__(SEQ_BLOCK) sequence_sum_kernel(
+template <int BLOCK>
+__global__ void __launch_bounds__(BLOCK) sequence_sum_kernel(
     const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
     bool average, float* __restrict__ out) {
-  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  __shared__ double smem[2 * BLOCK / WAVE_SIZE];
   long begin, end;
   seqs.span(blockIdx.x, begin, end);
-  double sum, count;
-  sum_span(lp, labels, ignore, begin, end, smem, sum, count);
-  if (threadIdx.x == 0) out[blockIdx.x] = (float)(average ? sum / fmax(count, 1.0) : sum);
+  double v[2];  // sum and number
+  sum_span<BLOCK>(lp, labels, ignore, begin, end, v[0], v[1]);
+  block_sums<BLOCK>(v, smem);
+  if (threadIdx.x == 0) out[blockIdx.x] = (float)(average ? v[0] / fmax(v[1], 1.0) : v[0]);
 }
 
 // coef of each row of a sequence from the gradient of the sequence's sum
-__global__ void __launch_bounds__(SEQ_BLOCK) sequence_coef_kernel(
+template <int BLOCK>
+__global__ void __launch_bounds__(BLOCK) sequence_coef_kernel(
     const float* __restrict__ grad, const long* __restrict__ labels, long ignore, Sequences seqs,
     bool average, float* __restrict__ coef) {
-  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  __shared__ double smem[BLOCK / WAVE_SIZE];
   long begin, end;
   seqs.span(blockIdx.x, begin, end);
-  double n = 0;
-  if (average)
-    for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) n += labels[r] != ignore ? 1.0 : 0.0;
-  n = block_sum<SEQ_BLOCK>(n, smem);
-  const float f = average ? (float)(grad[blockIdx.x] / fmax(n, 1.0)) : grad[blockIdx.x];
-  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) coef[r] = f;
+  double n[1] = {0};
+  if (average) {
+    for (long r = begin + threadIdx.x; r < end; r += BLOCK) n[0] += labels[r] != ignore ? 1.0 : 0.0;
+    block_sums<BLOCK>(n, smem);
+  }
+  const float f = average ? (float)(grad[blockIdx.x] / fmax(n[0], 1.0)) : grad[blockIdx.x];
+  for (long r = begin + threadIdx.x; r < end; r += BLOCK) coef[r] = f;
 }
 
 // True on the block that comes last, on all its threads; what the others wrote before is then visible to it.
@@ -388,24 +462,28 @@ __device__ __forceinline__ double read_shared(const double* p) {
 // The sums and d are kept in 64 bits: d is a small difference of large sums.
 enum { SIGMOID = 0, IPO = 1, HINGE = 2 };
 
-__global__ void __launch_bounds__(SEQ_BLOCK) preference_kernel(
+template <int BLOCK>
+__global__ void __launch_bounds__(BLOCK) preference_kernel(
     const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
     const float* __restrict__ ref, long pairs, int kind, double beta, double smoothing, bool average,
     float* __restrict__ coef, float* __restrict__ rewards, double* __restrict__ partial,
     int* __restrict__ arrived, float* __restrict__ loss_out) {
-  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  __shared__ double smem[4 * BLOCK / WAVE_SIZE];
   __shared__ int last;
   const long b = blockIdx.x;
   long begin[2], end[2];
-  double sum[2], count[2];
+  double v[4], count[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     seqs.span(b + k * pairs, begin[k], end[k]);
-    sum_span(lp, labels, ignore, begin[k], end[k], smem, sum[k], count[k]);
-    count[k] = average ? fmax(count[k], 1.0) : 1.0;
+    sum_span<BLOCK>(lp, labels, ignore, begin[k], end[k], v[k], v[2 + k]);
   }
-  const double chosen = sum[0] / count[0] - (double)ref[b];
-  const double rejected = sum[1] / count[1] - (double)ref[b + pairs];
+  const double ref_chosen = ref[b], ref_rejected = ref[b + pairs];
+  block_sums<BLOCK>(v, smem);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) count[k] = average ? fmax(v[2 + k], 1.0) : 1.0;
+  const double chosen = v[0] / count[0] - ref_chosen;
+  const double rejected = v[1] / count[1] - ref_rejected;
   const double d = chosen - rejected, z = beta * d;
   double loss, slope;  // slope = dloss/dd
   if (kind == SIGMOID) {
@@ -427,7 +505,7 @@ __global__ void __launch_bounds__(SEQ_BLOCK) preference_kernel(
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float f = (float)((k ? -slope : slope) / (count[k] * (double)pairs));
-    for (long r = begin[k] + threadIdx.x; r < end[k]; r += SEQ_BLOCK) coef[r] = f;
+    for (long r = begin[k] + threadIdx.x; r < end[k]; r += BLOCK) coef[r] = f;
   }
   if (threadIdx.x == 0) {
     rewards[b] = (float)(beta * chosen);
@@ -435,10 +513,10 @@ __global__ void __launch_bounds__(SEQ_BLOCK) preference_kernel(
     partial[b] = loss;
   }
   if (!comes_last(arrived, gridDim.x, &last)) return;
-  double total = 0;
-  for (long i = threadIdx.x; i < pairs; i += SEQ_BLOCK) total += read_shared(partial + i);
-  total = block_sum<SEQ_BLOCK>(total, smem);
-  if (threadIdx.x == 0) *loss_out = (float)(total / (double)pairs);
+  double total[1] = {0};
+  for (long i = threadIdx.x; i < pairs; i += BLOCK) total[0] += read_shared(partial + i);
+  block_sums<BLOCK>(total, smem);
+  if (threadIdx.x == 0) *loss_out = (float)(total[0] / (double)pairs);
 }
 
 // ---------------- clipped policy loss ----------------
@@ -468,45 +546,52 @@ enum { TOKEN = 0, SEQUENCE = 1, SUM = 2, NONE = 3 };
 
 // One block a sequence. `coef` comes without the division by the number of all
 // tokens (TOKEN): that number is known at the end only and goes out as `norm`.
-__global__ void __launch_bounds__(SEQ_BLOCK) policy_kernel(
+template <int BLOCK>
+__global__ void __launch_bounds__(BLOCK) policy_kernel(
     const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
     Policy policy, int reduction, float* __restrict__ coef, float* __restrict__ losses,
     double* __restrict__ partial, int* __restrict__ arrived, float* __restrict__ norm,
     float* __restrict__ loss_out) {
-  __shared__ double smem[SEQ_BLOCK / WAVE_SIZE];
+  __shared__ double smem[2 * BLOCK / WAVE_SIZE];
   __shared__ int last;
   const long s = blockIdx.x;
   long begin, end;
   seqs.span(s, begin, end);
-  double n = 0, sum = 0;
-  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) n += labels[r] != ignore ? 1.0 : 0.0;
-  n = block_sum<SEQ_BLOCK>(n, smem);
-  const double weight = reduction == SEQUENCE ? 1.0 / (fmax(n, 1.0) * (double)gridDim.x) : 1.0;
-  for (long r = begin + threadIdx.x; r < end; r += SEQ_BLOCK) {
+  double weight = 1.0;
+  if (reduction == SEQUENCE) {  // its number of tokens has to be known first
+    double n[1] = {0};
+    for (long r = begin + threadIdx.x; r < end; r += BLOCK) n[0] += labels[r] != ignore ? 1.0 : 0.0;
+    block_sums<BLOCK>(n, smem);
+    weight = 1.0 / (fmax(n[0], 1.0) * (double)gridDim.x);
+  }
+  double v[2] = {0, 0};  // loss and number of tokens
+  for (long r = begin + threadIdx.x; r < end; r += BLOCK) {
     float loss = 0.f, slope = 0.f;
-    if (labels[r] != ignore) loss = policy.of(lp[r], r, s, slope);
+    if (labels[r] != ignore) {
+      loss = policy.of(lp[r], r, s, slope);
+      v[1] += 1.0;
+    }
     coef[r] = (float)(weight * slope);
     if (reduction == NONE) losses[r] = loss;
-    sum += weight * loss;
+    v[0] += weight * loss;
   }
   if (reduction == NONE) return;
-  sum = block_sum<SEQ_BLOCK>(sum, smem);
+  block_sums<BLOCK>(v, smem);
   if (threadIdx.x == 0) {
-    partial[2 * s] = sum;
-    partial[2 * s + 1] = n;
+    partial[2 * s] = v[0];
+    partial[2 * s + 1] = v[1];
   }
   if (!comes_last(arrived, gridDim.x, &last)) return;
-  double total = 0, tokens = 0;
-  for (long i = threadIdx.x; i < gridDim.x; i += SEQ_BLOCK) {
-    total += read_shared(partial + 2 * i);
-    tokens += read_shared(partial + 2 * i + 1);
+  v[0] = v[1] = 0;
+  for (long i = threadIdx.x; i < gridDim.x; i += BLOCK) {
+    v[0] += read_shared(partial + 2 * i);
+    v[1] += read_shared(partial + 2 * i + 1);
   }
-  total = block_sum<SEQ_BLOCK>(total, smem);
-  tokens = block_sum<SEQ_BLOCK>(tokens, smem);
+  block_sums<BLOCK>(v, smem);
   if (threadIdx.x == 0) {
-    const double by = reduction == TOKEN ? 1.0 / fmax(tokens, 1.0) : 1.0;
+    const double by = reduction == TOKEN ? 1.0 / fmax(v[1], 1.0) : 1.0;
     *norm = (float)by;
-    *loss_out = (float)(total * by);
+    *loss_out = (float)(v[0] * by);
   }
 }
 
@@ -534,9 +619,10 @@ __global__ void __launch_bounds__(PREPARE_BLOCK) policy_prepare_kernel(
 #pragma unroll 4
     for (long r = begin + threadIdx.x; r < end; r += PREPARE_BLOCK) n += labels[r] != ignore ? 1 : 0;
   }
-  const double all = block_sum<PREPARE_BLOCK>((double)n, smem);
+  double all[1] = {(double)n};
+  block_sums<PREPARE_BLOCK>(all, smem);
   if (threadIdx.x == 0)
-    weights[blockIdx.x] = (float)(reduction == SUM ? 1.0 : 1.0 / (fmax(all, 1.0) * (reduction == SEQUENCE ? (double)count : 1.0)));
+    weights[blockIdx.x] = (float)(reduction == SUM ? 1.0 : 1.0 / (fmax(all[0], 1.0) * (reduction == SEQUENCE ? (double)count : 1.0)));
 }
 
 // One block a row, at most NP packs a lane and more than NP - 2: all but the last
@@ -621,15 +707,16 @@ __global__ void __launch_bounds__(TOTAL_BLOCK) total_kernel(const float* __restr
                                                             float* __restrict__ loss_out) {
   __shared__ double smem[TOTAL_BLOCK / WAVE_SIZE];
   __shared__ int last;
-  double sum = 0;
-  for (long r = (long)blockIdx.x * TOTAL_BLOCK + threadIdx.x; r < rows; r += (long)gridDim.x * TOTAL_BLOCK) sum += losses[r];
-  sum = block_sum<TOTAL_BLOCK>(sum, smem);
+  double sum[1] = {0};
+  for (long r = (long)blockIdx.x * TOTAL_BLOCK + threadIdx.x; r < rows; r += (long)gridDim.x * TOTAL_BLOCK) sum[0] += losses[r];
+  block_sums<TOTAL_BLOCK>(sum, smem);
   if (gridDim.x > 1) {
-    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum[0];
     if (!comes_last(arrived, gridDim.x, &last)) return;
-    sum = block_sum<TOTAL_BLOCK>(threadIdx.x < gridDim.x ? read_shared(partial + threadIdx.x) : 0.0, smem);
+    sum[0] = threadIdx.x < gridDim.x ? read_shared(partial + threadIdx.x) : 0.0;
+    block_sums<TOTAL_BLOCK>(sum, smem);
   }
-  if (threadIdx.x == 0) *loss_out = (float)sum;
+  if (threadIdx.x == 0) *loss_out = (float)sum[0];
 }
 
 // A gradient made for `applied` becomes that for *scale. Most often they are the same and nothing is moved.
@@ -726,16 +813,49 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
                   float2* stats, float* lp, int* arrived) {
   const Rows where = rows_of(logits);
   const long V = logits.size(-1), rows = labels.numel();
+  const Base c = base_of(temperature);
+  const long* y = labels.data_ptr<long>();
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
-    constexpr int BLOCK = 256;
-    hipLaunchKernelGGL((row_stats_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
-                       (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
-                       base_of(temperature), 1.0 / temperature, stats, lp, arrived);
+    const auto* x = (const scalar_t*)logits.data_ptr();
+    const long packs = V / Pack<scalar_t>::width;
+    // Up to 64 rows of 128 KB and more leave most of the chip without work: one to 64 rows of 131072 bf16 take 10.4
+    // to 11.5 us by blocks of a row each, 5.7 to 10.1 in parts. At half that length the second launch costs what it
+    // saves.
+    if (rows <= 64 && packs >= 8192) {
+      const int parts = (int)((packs + PART_PACKS - 1) / PART_PACKS);
+      auto room = at::empty({rows * parts, 2}, logits.options().dtype(at::kFloat));
+      auto* p = (float2*)room.data_ptr<float>();
+      hipLaunchKernelGGL((row_part_kernel<scalar_t>), dim3(parts, rows), dim3(PART_BLOCK), 0, current_stream(), x,
+                         where, y, ignore, V, c, p, arrived);
+      HIP_CHECK(hipGetLastError());
+      hipLaunchKernelGGL((row_join_kernel<scalar_t>), dim3(rows), dim3(WAVE_SIZE), 0, current_stream(), x, where, y,
+                         ignore, V, c, 1.0 / temperature, p, parts, stats, lp);
+      return;
+    }
+    auto launch = [&](auto block) {
+      constexpr int BLOCK = decltype(block)::value;
+      hipLaunchKernelGGL((row_stats_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
+                         x, where, y, ignore, V, rows, c, 1.0 / temperature, stats, lp, arrived);
+    };
+    // A block's cost is that of its start and of its join, which grow with its waves, and of its passes one after
+    // another. 8192 rows of 2048 bf16: 9.9 us by 64 lanes, 19.9 by 256; of 8192: 24.0 by 128, 28.7 by 256; of 32000:
+    // 86.9 by 256, 103 by 512; of 131072: 327 by 256, 310 by 512. Few rows wait for their passes, not for room: 512
+    // rows of 8192 5.5 by 128, 5.0 by 256.
+    using std::integral_constant;
+    if (packs <= 512) launch(integral_constant<int, 64>{});
+    else if (packs <= 1536 && rows >= 1024) launch(integral_constant<int, 128>{});
+    else if (packs < (rows >= 1024 ? 8192 : 3072)) launch(integral_constant<int, 256>{});
+    else launch(integral_constant<int, 512>{});
   }()));
   HIP_CHECK(hipGetLastError());
 }
 
-}  // namespace
+// Calls launch(block size) for blocks that have a sequence of `rows / count` rows each.
+template <typename F>
+void by_length(long rows, long count, F launch) {
+  if (rows / count > 512) launch(std::integral_constant<int, 1024>{});
+  else launch(std::integral_constant<int, 256>{});
+}
 
 // -> (lp, stats): stats [rows, 2] is what the backward pass needs of each row
 std::tuple<at::Tensor, at::Tensor> token_forward(at::Tensor logits, at::Tensor labels, long ignore,
@@ -791,8 +911,11 @@ std::tuple<at::Tensor, at::Tensor> sequence_forward(at::Tensor logits, at::Tenso
   if (labels.numel())
     launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), nullptr);
   if (count)
-    hipLaunchKernelGGL(sequence_sum_kernel, dim3(count), dim3(SEQ_BLOCK), 0, current_stream(),
-                       lp.data_ptr<float>(), labels.data_ptr<long>(), ignore, seqs, average, out.data_ptr<float>());
+    by_length(labels.numel(), count, [&](auto block) {
+      constexpr int BLOCK = decltype(block)::value;
+      hipLaunchKernelGGL((sequence_sum_kernel<BLOCK>), dim3(count), dim3(BLOCK), 0, current_stream(),
+                         lp.data_ptr<float>(), labels.data_ptr<long>(), ignore, seqs, average, out.data_ptr<float>());
+    });
   HIP_CHECK(hipGetLastError());
   return {out, stats};
 }
@@ -805,8 +928,11 @@ at::Tensor sequence_coef(at::Tensor grad, at::Tensor labels, c10::optional<at::T
   // rows behind the last packed sequence belong to none and get 0
   auto coef = cu ? at::zeros(labels.sizes(), grad.options()) : at::empty(labels.sizes(), grad.options());
   if (count)
-    hipLaunchKernelGGL(sequence_coef_kernel, dim3(count), dim3(SEQ_BLOCK), 0, current_stream(), g,
-                       labels.data_ptr<long>(), ignore, seqs, average, coef.data_ptr<float>());
+    by_length(labels.numel(), count, [&](auto block) {
+      constexpr int BLOCK = decltype(block)::value;
+      hipLaunchKernelGGL((sequence_coef_kernel<BLOCK>), dim3(count), dim3(BLOCK), 0, current_stream(), g,
+                         labels.data_ptr<long>(), ignore, seqs, average, coef.data_ptr<float>());
+    });
   HIP_CHECK(hipGetLastError());
   return coef;
 }
@@ -830,10 +956,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_forward(
   auto partial = at::empty({pairs + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
   int* arrived = (int*)(partial.data_ptr<double>() + pairs);
   launch_stats(logits, labels, ignore, 1.0, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), arrived);
-  hipLaunchKernelGGL(preference_kernel, dim3(pairs), dim3(SEQ_BLOCK), 0, current_stream(), lp.data_ptr<float>(),
-                     labels.data_ptr<long>(), ignore, seqs, rf, pairs, (int)kind, beta, smoothing, average,
-                     coef.data_ptr<float>(), rewards.data_ptr<float>(), partial.data_ptr<double>(), arrived,
-                     loss.data_ptr<float>());
+  by_length(rows, 2 * pairs, [&](auto block) {
+    constexpr int BLOCK = decltype(block)::value;
+    hipLaunchKernelGGL((preference_kernel<BLOCK>), dim3(pairs), dim3(BLOCK), 0, current_stream(), lp.data_ptr<float>(),
+                       labels.data_ptr<long>(), ignore, seqs, rf, pairs, (int)kind, beta, smoothing, average,
+                       coef.data_ptr<float>(), rewards.data_ptr<float>(), partial.data_ptr<double>(), arrived,
+                       loss.data_ptr<float>());
+  });
   HIP_CHECK(hipGetLastError());
   return {loss, rewards, stats, coef};
 }
@@ -861,10 +990,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_fo
   auto partial = at::empty({2 * count + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
   int* arrived = (int*)(partial.data_ptr<double>() + 2 * count);
   launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), arrived);
-  hipLaunchKernelGGL(policy_kernel, dim3(count), dim3(SEQ_BLOCK), 0, current_stream(), lp.data_ptr<float>(),
-                     labels.data_ptr<long>(), ignore, seqs, policy, (int)reduction, coef.data_ptr<float>(),
-                     loss.data_ptr<float>(), partial.data_ptr<double>(), arrived, norm.data_ptr<float>(),
-                     loss.data_ptr<float>());
+  by_length(rows, count, [&](auto block) {
+    constexpr int BLOCK = decltype(block)::value;
+    hipLaunchKernelGGL((policy_kernel<BLOCK>), dim3(count), dim3(BLOCK), 0, current_stream(), lp.data_ptr<float>(),
+                       labels.data_ptr<long>(), ignore, seqs, policy, (int)reduction, coef.data_ptr<float>(),
+                       loss.data_ptr<float>(), partial.data_ptr<double>(), arrived, norm.data_ptr<float>(),
+                       loss.data_ptr<float>());
+  });
   HIP_CHECK(hipGetLastError());
   return {loss, lp, stats, coef, norm};
 }
@@ -950,13 +1082,173 @@ void rescale_(at::Tensor grad, at::Tensor scale, at::Tensor applied) {
   HIP_CHECK(hipGetLastError());
 }
 
+// ---------------- autograd ----------------
+// In C++, so that the backward pass does not wait for the interpreter.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The gradient is not differentiable: said when it is differentiated, not when it is made.
+at::Tensor once(const char* name, at::Tensor grad) {
+  if (!at::GradMode::is_enabled()) return grad;
+  grad.set_requires_grad(true);
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " can be differentiated once only", 1);
+  return (*error)({grad})[0];
+}
+
+// What the gradient of the rows' log-probabilities becomes: kept between the passes
+void keep(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& stats,
+          const at::Tensor& coef, const at::Tensor& norm, long ignore, double temperature) {
+  ctx->save_for_backward({logits, labels, stats, coef, norm});
+  ctx->saved_data["ignore"] = (int64_t)ignore;
+  ctx->saved_data["temperature"] = temperature;
+  ctx->set_materialize_grads(false);
+}
+
+at::Tensor fp32(const at::Tensor& t) { return t.to(at::kFloat).contiguous(); }
+
+struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, int64_t ignore,
+                            double temperature) {
+    auto [lp, stats] = token_forward(logits, labels, ignore, temperature);
+    keep(ctx, logits, labels, stats, {}, {}, ignore, temperature);
+    return lp;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {{}, {}, {}, {}};
+    const auto saved = ctx->get_saved_variables();
+    auto grad = rows_backward(saved[0], saved[1], saved[2], fp32(grads[0].detach()), {}, {},
+                              ctx->saved_data["ignore"].toInt(), ctx->saved_data["temperature"].toDouble());
+    return {once("token_log_probs", grad), {}, {}, {}};
+  }
+};
+
+struct SequenceLogProbs : torch::autograd::Function<SequenceLogProbs> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels,
+                            const c10::optional<at::Tensor>& cu, int64_t count, bool average, int64_t ignore,
+                            double temperature) {
+    auto [sums, stats] = sequence_forward(logits, labels, cu, count, average, ignore, temperature);
+    keep(ctx, logits, labels, stats, cu ? *cu : at::Tensor(), {}, ignore, temperature);
+    ctx->saved_data["average"] = average;
+    return sums;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}};
+    const auto saved = ctx->get_saved_variables();
+    const long ignore = ctx->saved_data["ignore"].toInt();
+    const auto cu = saved[3].defined() ? c10::optional<at::Tensor>(saved[3]) : c10::nullopt;
+    auto coef = sequence_coef(fp32(grads[0].detach()), saved[1], cu, ctx->saved_data["average"].toBool(), ignore);
+    auto grad = rows_backward(saved[0], saved[1], saved[2], coef, {}, {}, ignore, ctx->saved_data["temperature"].toDouble());
+    return {once("sequence_log_probs", grad), {}, {}, {}, {}, {}, {}};
+  }
+};
+
+// The backward pass of a loss whose coefficients the forward pass has made
+at::Tensor loss_backward(const char* name, AutogradContext* ctx, const at::Tensor& given) {
+  const auto saved = ctx->get_saved_variables();
+  const auto norm = saved[4].defined() ? c10::optional<at::Tensor>(saved[4]) : c10::nullopt;
+  return once(name, rows_backward(saved[0], saved[1], saved[2], saved[3], fp32(given.detach()), norm,
+                                  ctx->saved_data["ignore"].toInt(), ctx->saved_data["temperature"].toDouble()));
+}
+
+struct PreferenceCall {
+  at::Tensor labels, ref;
+  c10::optional<at::Tensor> cu;
+  long pairs, kind;
+  double beta, smoothing;
+  bool average;
+  long ignore;
+};
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const PreferenceCall& a) {
+    auto [loss, rewards, stats, coef] = preference_forward(logits, a.labels, a.ref, a.cu, a.pairs, a.kind, a.beta,
+                                                           a.smoothing, a.average, a.ignore);
+    keep(ctx, logits, a.labels, stats, coef, {}, a.ignore, 1.0);
+    auto chosen = rewards.narrow(0, 0, a.pairs), rejected = rewards.narrow(0, a.pairs, a.pairs);
+    ctx->mark_non_differentiable({chosen, rejected});
+    return {loss, chosen, rejected};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {{}, {}};
+    return {loss_backward("preference_loss", ctx, grads[0]), {}};
+  }
+};
+
+struct PolicyCall {
+  at::Tensor labels, advantages;
+  c10::optional<at::Tensor> old, ref, cu, scale_tensor;
+  bool by_row;
+  long count, reduction, ignore;
+  double low, high, kl, temperature, scale;
+};
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const PolicyCall& a) {
+    auto [loss, lp, stats, coef, norm] = policy_forward(logits, a.labels, a.old, a.advantages, a.by_row, a.ref, a.cu,
+                                                        a.count, a.low, a.high, a.kl, a.temperature, a.reduction, a.ignore);
+    keep(ctx, logits, a.labels, stats, coef, a.reduction == TOKEN ? norm : at::Tensor(), a.ignore, a.temperature);
+    ctx->mark_non_differentiable({lp});
+    return {loss, lp};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {{}, {}};
+    return {loss_backward("policy_loss", ctx, grads[0]), {}};
+  }
+};
+
+// The loss and, in the same pass over the logits, their gradient for a gradient of the loss that is known
+struct PolicyLossAtOnce : torch::autograd::Function<PolicyLossAtOnce> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const PolicyCall& a) {
+    auto [loss, lp, grad, applied] = policy_at_once(logits, a.labels, a.old, a.advantages, a.by_row, a.ref, a.cu, a.count,
+                                                    a.low, a.high, a.kl, a.temperature, a.reduction, a.ignore, a.scale,
+                                                    a.scale_tensor);
+    ctx->saved_data["grad"] = grad;
+    ctx->saved_data["applied"] = applied;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({lp});
+    return {loss, lp};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {{}, {}};
+    TORCH_CHECK(ctx->saved_data.count("grad"),
+                "policy_loss(grad_scale=...) made its gradient in the forward pass: it can be taken once only");
+    auto grad = ctx->saved_data["grad"].toTensor();
+    rescale_(grad, fp32(grads[0].detach()), ctx->saved_data["applied"].toTensor());
+    ctx->saved_data.erase("grad");
+    return {once("policy_loss", grad), {}};
+  }
+};
+
+at::Tensor token_log_probs(at::Tensor logits, at::Tensor labels, long ignore, double temperature) {
+  return TokenLogProbs::apply(logits, labels, (int64_t)ignore, temperature);
+}
+
+at::Tensor sequence_log_probs(at::Tensor logits, at::Tensor labels, c10::optional<at::Tensor> cu, long count,
+                              bool average, long ignore, double temperature) {
+  return SequenceLogProbs::apply(logits, labels, cu, (int64_t)count, average, (int64_t)ignore, temperature);
+}
+
+variable_list preference_loss(at::Tensor logits, at::Tensor labels, at::Tensor ref, c10::optional<at::Tensor> cu,
+                              long pairs, long kind, double beta, double smoothing, bool average, long ignore) {
+  return PreferenceLoss::apply(logits, PreferenceCall{labels, ref, cu, pairs, kind, beta, smoothing, average, ignore});
+}
+
+variable_list policy_loss(at::Tensor logits, at::Tensor labels, c10::optional<at::Tensor> old, at::Tensor advantages,
+                          bool by_row, c10::optional<at::Tensor> ref, c10::optional<at::Tensor> cu, long count,
+                          double low, double high, double kl, double temperature, long reduction, long ignore,
+                          bool at_once, double scale, c10::optional<at::Tensor> scale_tensor) {
+  const PolicyCall a{labels, advantages, old, ref, cu, scale_tensor, by_row, count, reduction, ignore,
+                     low, high, kl, temperature, scale};
+  // without a backward pass there is no gradient to make
+  if (at_once && logits.requires_grad() && at::GradMode::is_enabled()) return PolicyLossAtOnce::apply(logits, a);
+  return PolicyLoss::apply(logits, a);
+}
+
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("token_forward", &token_forward, "log-probabilities of given tokens -> (lp, stats)");
-  m.def("rows_backward", &rows_backward, "logits' gradient from that of the log-probabilities");
-  m.def("sequence_forward", &sequence_forward, "sequences' log-probabilities -> (sums, stats)");
-  m.def("sequence_coef", &sequence_coef, "gradient of each token from that of its sequence");
-  m.def("preference_forward", &preference_forward, "paired log ratios -> (loss, rewards, stats, coef)");
-  m.def("policy_forward", &policy_forward, "clipped policy loss with KL -> (loss, lp, stats, coef, norm)");
-  m.def("policy_at_once", &policy_at_once, "the policy loss and the logits' gradient -> (loss, lp, dlogits, applied)");
-  m.def("rescale_", &rescale_, "a gradient made for one gradient of the loss becomes that for another");
+  m.def("token_log_probs", &token_log_probs, "log-probabilities of given tokens");
+  m.def("sequence_log_probs", &sequence_log_probs, "log-probabilities of sequences");
+  m.def("preference_loss", &preference_loss, "paired log ratios -> (loss, chosen rewards, rejected rewards)");
+  m.def("policy_loss", &policy_loss, "clipped policy loss with KL -> (loss, log-probabilities)");
 }

@@ -430,3 +430,39 @@ def test_a_change_in_place_is_noticed():
     x.add_(1)
     with pytest.raises(RuntimeError, match="modified"):
         lp.sum().backward()
+
+
+def test_gradients_are_differentiable_once():
+    x, y, _ = make((4, 5), 12, torch.float32, ignored=0)
+    x = x.cuda().requires_grad_(True)
+    w = torch.ones(4, 5, device="cuda", requires_grad=True)
+    g = torch.autograd.grad(token_log_probs(x, y.cuda()), x, w, create_graph=True)[0]
+    assert torch.isfinite(g).all()
+    with pytest.raises(RuntimeError, match="once only"):
+        g.sum().backward()
+
+
+def test_outputs_without_a_gradient():
+    """Rewards and log-probabilities are not differentiable; a loss that nothing asks for leaves no gradient."""
+    x, y, _ = make((4, 5), 12, torch.float32, ignored=0)
+    x = x.cuda().requires_grad_(True)
+    loss, chosen, rejected = preference_loss(x, y.cuda(), torch.zeros(4, device="cuda"))
+    assert loss.requires_grad and not chosen.requires_grad and not rejected.requires_grad
+    loss, lp = policy_loss(x, y.cuda(), None, torch.ones(4, device="cuda"))
+    assert loss.requires_grad and not lp.requires_grad
+    (chosen.sum() + rejected.sum() + lp.sum() + x.sum()).backward()
+    assert (x.grad == 1).all()
+    with torch.no_grad():
+        assert not policy_loss(x, y.cuda(), None, torch.ones(4, device="cuda"))[0].requires_grad
+
+
+def test_gradients_add_up_over_calls():
+    """Two calls on one leaf, a loss of both: AccumulateGrad and the sum of the two gradients."""
+    x, y, _ = make((4, 5), 300, torch.float32, ignored=0)
+    ref = torch.zeros(4, device="cuda")
+    a, b = x.cuda().requires_grad_(True), x.cuda().requires_grad_(True)
+    la, lb = preference_loss(a, y.cuda(), ref)[0], policy_loss(a, y.cuda(), None, ref + 1, grad_scale=1.0)[0]
+    (la + lb).backward()
+    want = torch.autograd.grad(preference_loss(b, y.cuda(), ref)[0], b)[0] + torch.autograd.grad(policy_loss(b, y.cuda(), None, ref + 1)[0], b)[0]
+    # fp32 sums of two values under 1, each within some half steps
+    torch.testing.assert_close(a.grad, want, rtol=0, atol=8 * 2 ** -24)
