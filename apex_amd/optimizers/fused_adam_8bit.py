@@ -21,6 +21,7 @@ from ..tracing import traced
 BLOCK = 128  # elements of one scale
 _E4M3_MAX = 448.0
 _MASK = 0xFFFFFFFF
+_STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
 
 
 def _mix(x):
@@ -147,18 +148,17 @@ class FusedAdam8bit(torch.optim.Optimizer):
                     if torch.is_tensor(group.get(key)):
                         group[key] = group[key].item()
 
-    def _state(self, p):
-        state = self.state[p]
-        if len(state) == 0:
-            if torch.empty_like(p, device="meta").stride() != p.stride():
-                raise RuntimeError("FusedAdam8bit only supports dense params without gaps or overlaps")
-            blocks = -(-p.numel() // BLOCK)
-            for name in ("exp_avg", "exp_avg_sq"):
-                state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
-                state[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-            if self.master_weights and p.dtype != torch.float32:
-                state["master_param"] = p.detach().float().clone()
-        return state
+    def _init_state(self, p, state):
+        if p.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise RuntimeError("FusedAdam8bit only supports fp16/bf16/fp32 params")
+        if torch.empty_like(p, device="meta").stride() != p.stride():
+            raise RuntimeError("FusedAdam8bit only supports dense params without gaps or overlaps")
+        blocks = -(-p.numel() // BLOCK)
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
+            state[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        if self.master_weights and p.dtype != torch.float32:
+            state["master_param"] = p.detach().float().clone()
 
     @torch.no_grad()
     @traced("FusedAdam8bit.step")
@@ -170,33 +170,37 @@ class FusedAdam8bit(torch.optim.Optimizer):
 
         first = 0  # a tensor's place in the optimizer is part of its random numbers
         for group in self.param_groups:
-            place, first = first, first + len(group["params"])
-            lists = {}  # by device, dtype and whether there is a master copy
-            for i, p in enumerate(group["params"]):
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("FusedAdam8bit does not support sparse gradients")
-                if p.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-                    raise RuntimeError("FusedAdam8bit only supports fp16/bf16/fp32 params")
-                state = self._state(p)
-                grad = p.grad
-                if grad.stride() != p.stride():  # elements are met in memory order
-                    grad = torch.empty_like(p).copy_(grad)
-                row = [grad, p, state["exp_avg"], state["exp_avg_scale"], state["exp_avg_sq"], state["exp_avg_sq_scale"]]
-                if "master_param" in state:
-                    row.append(state["master_param"])
-                lists.setdefault((p.device, p.dtype, len(row)), []).append((place + i, row))
-            if not group["params"]:
+            params = group["params"]
+            if not params:
                 continue
+            lists = {}  # by device, dtype and whether there is a master copy
+            for place, p in enumerate(params, first):
+                grad = p.grad
+                if grad is None:
+                    continue
+                if grad.is_sparse:
+                    raise RuntimeError("FusedAdam8bit does not support sparse gradients")
+                state = self.state[p]
+                if not state:
+                    self._init_state(p, state)
+                key = p.device, p.dtype, "master_param" in state
+                row = place, grad, p, state
+                if key in lists:
+                    lists[key].append(row)
+                else:
+                    lists[key] = [row]
+            first += len(params)
             found_inf, inv_scale = self._count(group, grad_scaler)
-            for (device, _, _), rows in lists.items():
-                places, tensors = [i for i, _ in rows], [list(t) for t in zip(*(r for _, r in rows))]
+            for (device, _, master), rows in lists.items():
+                names = _STATE + (("master_param",) if master else ())
                 if device.type == "cuda":
-                    self._step_cuda(group, places, tensors, found_inf, inv_scale)
+                    tensors = [[r[1] for r in rows], [r[2] for r in rows]] + [[r[3][name] for r in rows] for name in names]
+                    self._step_cuda(group, [r[0] for r in rows], tensors, found_inf, inv_scale)
                 elif found_inf is None or not float(found_inf):
-                    for i, row in zip(places, zip(*tensors)):
-                        self._step_ref(group, i, inv_scale, *row)
+                    for place, grad, p, state in rows:
+                        if grad.stride() != p.stride():  # elements are met in memory order
+                            grad = torch.empty_like(p).copy_(grad)
+                        self._step_ref(group, place, inv_scale, grad, p, *(state[name] for name in names))
         return loss
 
     def _count(self, group, grad_scaler):

@@ -370,7 +370,7 @@ Adam8Args args_of(double beta1, double beta2, double eps, long mode, long bias_c
 }
 
 // tensor_lists: g, p, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale(, master)
-void adam_8bit(const TensorLists& lists, const std::vector<long>& ordinals, const Adam8Args& args) {
+void adam_8bit(TensorLists& lists, const std::vector<long>& ordinals, const Adam8Args& args) {
   TORCH_CHECK(lists.size() == 6 || lists.size() == 7, "multi_tensor_adam_8bit: 6 lists, or 7 with master weights");
   const size_t count = lists[0].size();
   const bool master = lists.size() == 7;
@@ -387,6 +387,9 @@ void adam_8bit(const TensorLists& lists, const std::vector<long>& ordinals, cons
     int nt = 0;
     long chunks = 0;
     while (t < count && nt < A8_TENSORS) {
+      // a gradient of another layout is met in the param's order; the copy lives until the launch is under way
+      if (lists[0][t].strides() != lists[1][t].strides() && lists[0][t].numel() > 1)
+        lists[0][t] = at::empty_like(lists[1][t]).copy_(lists[0][t]);
       const long n = lists[1][t].numel(), blocks = (n + A8_SCALE_BLOCK - 1) / A8_SCALE_BLOCK;
       for (size_t d = 0; d < lists.size(); ++d) {
         const auto& x = lists[d][t];
