@@ -68,8 +68,26 @@ struct Pack {
   T a[width];
 };
 
-// 16 bytes at an address that is aligned to its element only (rows of an odd V),
-// past the caches: nothing here is met twice in a pass
+// A row in packs that are aligned at `p`, and the elements before and behind them:
+// rows of an odd V begin anywhere, and packs that lie across cache lines cost
+// (rows of 50257 bf16, loads and stores: 5.4 TB/s, of 50304 6.1).
+struct Packs {
+  int head, whole, singles;  // elements before, packs, elements before and behind
+  template <typename T>
+  __device__ __forceinline__ static Packs of(const T* p, long V) {
+    constexpr int W = 16 / sizeof(T);
+    const int head = (int)min((long)((16 - ((unsigned long)p & 15)) & 15) / (long)sizeof(T), V);
+    const int whole = (int)((V - head) / W);
+    return {head, whole, (int)(V - (long)whole * W)};
+  }
+  // the element of single j, and whether (and where) the label is one
+  __device__ __forceinline__ int single(int j, int W) const { return j < head ? j : whole * W + j; }
+  __device__ __forceinline__ bool is_single(long y, int W) const { return y < head || y >= head + (long)whole * W; }
+};
+
+// 16 bytes at an address that is aligned to its element only (rows that lie
+// otherwise than the gradient's), past the caches: nothing here is met twice in a
+// pass
 typedef unsigned wide __attribute__((ext_vector_type(4)));
 typedef unsigned wide_at_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned wide_at_2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -193,6 +211,26 @@ __device__ __forceinline__ float log_prob(float x, Running w, double inv_t, floa
   return (float)((double)(x - w.m) * inv_t - 0.6931471805599453 * (double)log2s);
 }
 
+// What a row's pass leaves: its statistics, and its log-probability in 32 bits, or
+// in 64 where many of them are going to be added and a small difference of the
+// sums is asked for.
+struct RowOut {
+  float2* stats;
+  float* lp;
+  double* lp64;
+  __device__ __forceinline__ void none(long row, float value) const {
+    stats[row] = make_float2(value, value);
+    if (lp64) lp64[row] = value;
+    else lp[row] = value;
+  }
+  __device__ __forceinline__ void put(long row, float x, Running w, double inv_t) const {
+    const float l2 = log2f(w.s);
+    stats[row] = make_float2(w.m, l2);
+    if (lp64) lp64[row] = (double)(x - w.m) * inv_t - log((double)w.s);
+    else lp[row] = log_prob(x, w, inv_t, l2);
+  }
+};
+
 // A block's sums of N values in 64 bits, in a fixed order; valid on every thread.
 template <int BLOCK, int N>
 __device__ __forceinline__ void block_sums(double (&v)[N], double* smem /* N * waves */) {
@@ -220,25 +258,24 @@ constexpr int UNROLL = 4;  // packs of a lane that are on their way together
 template <typename T, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) row_stats_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
-    long rows, Base c, double inv_t, float2* __restrict__ stats, float* __restrict__ lp_out,
-    int* __restrict__ arrived) {
+    long rows, Base c, double inv_t, RowOut out, int* __restrict__ arrived) {
   __shared__ float smem[2 * (BLOCK / WAVE_SIZE)];
   constexpr int W = Pack<T>::width;
   if (arrived && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // for the kernel after this one
-  const long whole = V / W;
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     const long y = labels[row];
     if (y == ignore || y < 0 || y >= V) {
-      if (threadIdx.x == 0) {
-        const float none = y == ignore ? 0.f : NAN;
-        lp_out[row] = none;
-        stats[row] = make_float2(none, none);
-      }
+      if (threadIdx.x == 0) out.none(row, y == ignore ? 0.f : NAN);
       continue;
     }
-    const T* x = logits + where.at(row);
+    const T* first = logits + where.at(row);
+    const Packs in = Packs::of(first, V);
+    const T* x = first + in.head;
+    const int whole = in.whole;
     Running w;
-    long k = threadIdx.x;
+    T single = from_float<T>(-INFINITY);
+    if ((int)threadIdx.x < in.singles) single = first[in.single(threadIdx.x, W)];
+    int k = threadIdx.x;
     for (; k + (UNROLL - 1) * BLOCK < whole; k += UNROLL * BLOCK) {
       Pack<T> v[UNROLL];
 #pragma unroll
@@ -253,17 +290,10 @@ __global__ void __launch_bounds__(BLOCK) row_stats_kernel(
       for (int u = 0; u < UNROLL - 1; ++u)
         if (k + u * BLOCK < whole) take<T, 1>(w, v + u, c);
     }
-    if (const long i = whole * W + threadIdx.x; i < V) {
-      const float f = to_float(x[i]);
-      w.raise(f, c);
-      w.s += c.exp(f - w.origin());
-    }
+    w.raise(to_float(single), c);
+    w.s += c.exp(to_float(single) - w.origin());
     w = block_join<BLOCK>(w, c, smem);
-    if (threadIdx.x == 0) {
-      const float l2 = log2f(w.s);
-      lp_out[row] = log_prob(to_float(x[y]), w, inv_t, l2);
-      stats[row] = make_float2(w.m, l2);
-    }
+    if (threadIdx.x == 0) out.put(row, to_float(first[y]), w, inv_t);
     __syncthreads();  // smem is the next row's
   }
 }
@@ -303,15 +333,10 @@ __global__ void __launch_bounds__(PART_BLOCK) row_part_kernel(
 template <typename T>
 __global__ void __launch_bounds__(WAVE_SIZE) row_join_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V, Base c,
-    double inv_t, const float2* __restrict__ parts, int count, float2* __restrict__ stats,
-    float* __restrict__ lp_out) {
+    double inv_t, const float2* __restrict__ parts, int count, RowOut out) {
   const long row = blockIdx.x, y = labels[row];
   if (y == ignore || y < 0 || y >= V) {
-    if (threadIdx.x == 0) {
-      const float none = y == ignore ? 0.f : NAN;
-      lp_out[row] = none;
-      stats[row] = make_float2(none, none);
-    }
+    if (threadIdx.x == 0) out.none(row, y == ignore ? 0.f : NAN);
     return;
   }
   const float xy = to_float(logits[where.at(row) + y]);
@@ -322,11 +347,7 @@ __global__ void __launch_bounds__(WAVE_SIZE) row_join_kernel(
   }
 #pragma unroll
   for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) w.join(__shfl_xor(w.m, off), __shfl_xor(w.s, off), c);
-  if (threadIdx.x == 0) {
-    const float l2 = log2f(w.s);
-    lp_out[row] = log_prob(xy, w, inv_t, l2);
-    stats[row] = make_float2(w.m, l2);
-  }
+  if (threadIdx.x == 0) out.put(row, xy, w, inv_t);
 }
 
 // ---------------- rows: gradient ----------------
@@ -366,27 +387,30 @@ __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
     const float* __restrict__ scale, long scale_stride, const float* __restrict__ norm,
     T* __restrict__ grad) {
   constexpr int W = Pack<T>::width;
-  const long whole = V / W, k = (long)blockIdx.x * BLOCK + threadIdx.x;
-  // lanes behind the row's last pack have the elements that make no pack, one each
-  const long i = k < whole ? k * W : whole * W + (k - whole);
+  const int k = blockIdx.x * BLOCK + threadIdx.x;
   for (long row = blockIdx.y; row < rows; row += gridDim.y) {
     const long y = labels[row];
     T* g = grad + row * V;
+    const Packs in = Packs::of(g, V);
+    // the row's first lanes have the elements that make no pack as well
+    const bool pack = k < in.whole, one = k < in.singles;
+    const int i = in.head + k * W, single = in.single(k, W);
     float f = coef[row] * inv_t;
     if (scale) f *= scale[row * scale_stride];
     if (norm) f *= *norm;
     if (y == ignore || f == 0.f) {  // a clipped token, or one that no sequence has: its logits are not asked
-      if (k < whole) store16(g + i, zeros<T>());
-      else if (i < V) g[i] = from_float<T>(0.f);
+      if (pack) store16(g + i, zeros<T>());
+      if (one) g[single] = from_float<T>(0.f);
       continue;
     }
     const T* x = logits + where.at(row);
     const float2 st = stats[row];
     const Gradient d{f, st.x, st.y, c};
-    if (k < whole) d.put(load16(x + i), g + i);
-    else if (i < V) g[i] = from_float<T>(-f * d.p(to_float(x[i])));
+    if (pack) d.put(load16(x + i), g + i);
+    if (one) g[single] = from_float<T>(-f * d.p(to_float(x[single])));
     // the label's element, by the lane that has just written its pack
-    if (y >= 0 && y < V && (k < whole ? y >= i && y < i + W : y == i)) g[y] = from_float<T>(d.at_label(to_float(x[y])));
+    if (y >= 0 && y < V && ((pack && y >= i && y < i + W) || (one && y == single)))
+      g[y] = from_float<T>(d.at_label(to_float(x[y])));
   }
 }
 
@@ -395,21 +419,21 @@ __global__ void __launch_bounds__(BLOCK) row_grad_kernel(
 
 // A lane's sum (in 64 bits) and number of a sequence's labelled lp.
 template <int BLOCK>
-__device__ __forceinline__ void sum_span(const float* lp, const long* labels, long ignore, long begin,
+__device__ __forceinline__ void sum_span(const double* lp, const long* labels, long ignore, long begin,
                                          long end, double& sum, double& count) {
   sum = count = 0;
 #pragma unroll 2
   for (long r = begin + threadIdx.x; r < end; r += BLOCK) {
-    const float v = lp[r];
+    const double v = lp[r];
     const bool on = labels[r] != ignore;
-    sum += on ? (double)v : 0.0;
+    sum += on ? v : 0.0;
     count += on ? 1.0 : 0.0;
   }
 }
 
 template <int BLOCK>
 __global__ void __launch_bounds__(BLOCK) sequence_sum_kernel(
-    const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
+    const double* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
     bool average, float* __restrict__ out) {
   __shared__ double smem[2 * BLOCK / WAVE_SIZE];
   long begin, end;
@@ -464,7 +488,7 @@ enum { SIGMOID = 0, IPO = 1, HINGE = 2 };
 
 template <int BLOCK>
 __global__ void __launch_bounds__(BLOCK) preference_kernel(
-    const float* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
+    const double* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
     const float* __restrict__ ref, long pairs, int kind, double beta, double smoothing, bool average,
     float* __restrict__ coef, float* __restrict__ rewards, double* __restrict__ partial,
     int* __restrict__ arrived, float* __restrict__ loss_out) {
@@ -625,8 +649,8 @@ __global__ void __launch_bounds__(PREPARE_BLOCK) policy_prepare_kernel(
     weights[blockIdx.x] = (float)(reduction == SUM ? 1.0 : 1.0 / (fmax(all[0], 1.0) * (reduction == SEQUENCE ? (double)count : 1.0)));
 }
 
-// One block a row, at most NP packs a lane and more than NP - 2: all but the last
-// two are there without a question.
+// One block a row, at most NP packs a lane and NP - 2 of each at least: only the
+// last two are asked for.
 template <typename T, int BLOCK, int NP>
 __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V, long first_row,
@@ -638,10 +662,13 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
   const long row = first_row + blockIdx.x;
   const long y = labels[row];
   T* g = grad + row * V;
-  const int whole = (int)(V / W), tail = whole * W + (int)threadIdx.x, lane = threadIdx.x * W;
+  const Packs in = Packs::of(g, V);
+  const int whole = in.whole, lane = in.head + (int)threadIdx.x * W;
+  const bool one = (int)threadIdx.x < in.singles;
+  const int single = in.single(threadIdx.x, W);
   const auto put_zeros = [&] {
-    for (int k = threadIdx.x; k < whole; k += BLOCK) store16(g + k * W, zeros<T>());
-    if (tail < V) g[tail] = from_float<T>(0.f);
+    for (int k = threadIdx.x; k < whole; k += BLOCK) store16(g + in.head + k * W, zeros<T>());
+    if (one) g[single] = from_float<T>(0.f);
   };
   if (y == ignore) {
     if (threadIdx.x == 0) lp_out[row] = losses[row] = 0.f;
@@ -649,15 +676,15 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
     return;
   }
   const T* x = logits + where.at(row);
-  const bool in = y >= 0 && y < V;
-  const T xy = x[in ? y : 0];
+  const bool valid = y >= 0 && y < V;
+  const T xy = x[valid ? y : 0];
   const bool has[2] = {(NP - 2) * BLOCK + (int)threadIdx.x < whole, (NP - 1) * BLOCK + (int)threadIdx.x < whole};
   wide v[NP];
 #pragma unroll
   for (int u = 0; u < NP; ++u)
     if (u < NP - 2 || has[u - (NP - 2)]) v[u] = load_wide(x + u * BLOCK * W + lane);
   T xt = from_float<T>(-INFINITY);
-  if (tail < V) xt = x[tail];
+  if (one) xt = x[single];
   Running w;
 #pragma unroll
   for (int u = 0; u < NP; ++u)
@@ -669,7 +696,7 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
   w.raise(to_float(xt), c);
   w.s += c.exp(to_float(xt) - w.origin());
   w = block_join<BLOCK>(w, c, smem);
-  const float l2 = log2f(w.s), lp = log_prob(in ? to_float(xy) : NAN, w, inv_t, l2);
+  const float l2 = log2f(w.s), lp = log_prob(valid ? to_float(xy) : NAN, w, inv_t, l2);
   float f = 0.f, loss = 0.f;
   const long s = owner_of(seqs, count, row);
   if (s >= 0) {
@@ -695,9 +722,10 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
       d.put(pack_of<T>(v[u]), g + u * BLOCK * W + lane);
       __builtin_amdgcn_sched_barrier(0);
     }
-  if (tail < V) g[tail] = from_float<T>(-f * d.p(to_float(xt)));
+  if (one) g[single] = from_float<T>(-f * d.p(to_float(xt)));
   // the label's element, by the lane that has just written its pack
-  if (in && (y < whole * W ? (y / W) % BLOCK == threadIdx.x : y == tail)) g[y] = from_float<T>(d.at_label(to_float(xy)));
+  if (valid && (in.is_single(y, W) ? one && y == single : (y - in.head) / W % BLOCK == threadIdx.x))
+    g[y] = from_float<T>(d.at_label(to_float(xy)));
 }
 
 // The rows' weighted losses, in a fixed order and 64 bits
@@ -776,7 +804,7 @@ void check_rows(const at::Tensor& logits, const at::Tensor& labels) {
   TORCH_CHECK(labels.device() == logits.device(), "token_loss: labels are on another device than the logits");
   TORCH_CHECK(labels.is_contiguous(), "token_loss: labels must be contiguous");
   TORCH_CHECK(labels.numel() * logits.size(-1) == logits.numel(), "token_loss: one label a row");
-  TORCH_CHECK(labels.numel() < std::numeric_limits<int>::max(), "token_loss: too many rows");
+  TORCH_CHECK(labels.numel() < std::numeric_limits<int>::max() && logits.size(-1) < (1L << 30), "token_loss: too many rows, or too long ones");
 }
 
 // fp32 and contiguous, on the logits' device, with n values
@@ -810,7 +838,10 @@ Policy policy_of(const at::Tensor& logits, const c10::optional<at::Tensor>& old,
 }
 
 void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, double temperature,
-                  float2* stats, float* lp, int* arrived) {
+                  const at::Tensor& stats, const at::Tensor& lp, int* arrived) {
+  const bool wide = lp.scalar_type() == at::kDouble;
+  const RowOut out{(float2*)stats.data_ptr<float>(), wide ? nullptr : lp.data_ptr<float>(),
+                   wide ? lp.data_ptr<double>() : nullptr};
   const Rows where = rows_of(logits);
   const long V = logits.size(-1), rows = labels.numel();
   const Base c = base_of(temperature);
@@ -829,13 +860,13 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
                          where, y, ignore, V, c, p, arrived);
       HIP_CHECK(hipGetLastError());
       hipLaunchKernelGGL((row_join_kernel<scalar_t>), dim3(rows), dim3(WAVE_SIZE), 0, current_stream(), x, where, y,
-                         ignore, V, c, 1.0 / temperature, p, parts, stats, lp);
+                         ignore, V, c, 1.0 / temperature, p, parts, out);
       return;
     }
     auto launch = [&](auto block) {
       constexpr int BLOCK = decltype(block)::value;
       hipLaunchKernelGGL((row_stats_kernel<scalar_t, BLOCK>), dim3(grid_of(rows)), dim3(BLOCK), 0, current_stream(),
-                         x, where, y, ignore, V, rows, c, 1.0 / temperature, stats, lp, arrived);
+                         x, where, y, ignore, V, rows, c, 1.0 / temperature, out, arrived);
     };
     // A block's cost is that of its start and of its join, which grow with its waves, and of its passes one after
     // another. 8192 rows of 2048 bf16: 9.9 us by 64 lanes, 19.9 by 256; of 8192: 24.0 by 128, 28.7 by 256; of 32000:
@@ -866,7 +897,7 @@ std::tuple<at::Tensor, at::Tensor> token_forward(at::Tensor logits, at::Tensor l
   auto lp = at::empty(labels.sizes(), opts);
   auto stats = at::empty({labels.numel(), 2}, opts);
   if (labels.numel())
-    launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), nullptr);
+    launch_stats(logits, labels, ignore, temperature, stats, lp, nullptr);
   return {lp, stats};
 }
 
@@ -885,13 +916,18 @@ at::Tensor rows_backward(at::Tensor logits, at::Tensor labels, at::Tensor stats,
   const float* no = norm ? floats(*norm, logits, 1, "norm") : nullptr;
   const long step = scale && scale->numel() == rows && rows > 1 ? 1 : 0;
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
-    constexpr int BLOCK = 256;
-    const long lanes = V / Pack<scalar_t>::width + V % Pack<scalar_t>::width;
-    const dim3 grid((lanes + BLOCK - 1) / BLOCK, std::min<long>(rows, 65535));
-    hipLaunchKernelGGL((row_grad_kernel<scalar_t, BLOCK>), grid, dim3(BLOCK), 0, current_stream(),
-                       (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
-                       (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature),
-                       (const float2*)st, co, sc, step, no, (scalar_t*)grad.data_ptr());
+    const long lanes = std::max(V / Pack<scalar_t>::width, 1L);
+    auto launch = [&](auto block) {
+      constexpr int BLOCK = decltype(block)::value;
+      const dim3 grid((lanes + BLOCK - 1) / BLOCK, std::min<long>(rows, 65535));
+      hipLaunchKernelGGL((row_grad_kernel<scalar_t, BLOCK>), grid, dim3(BLOCK), 0, current_stream(),
+                         (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
+                         (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature),
+                         (const float2*)st, co, sc, step, no, (scalar_t*)grad.data_ptr());
+    };
+    if (lanes <= 64) launch(std::integral_constant<int, 64>{});
+    else if (lanes <= 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, 256>{});
   }()));
   HIP_CHECK(hipGetLastError());
   return grad;
@@ -905,16 +941,16 @@ std::tuple<at::Tensor, at::Tensor> sequence_forward(at::Tensor logits, at::Tenso
   const at::DeviceGuard guard(logits.device());
   auto opts = logits.options().dtype(at::kFloat);
   const Sequences seqs = sequences_of(labels, cu, count);
-  auto lp = at::empty(labels.sizes(), opts);
+  auto lp = at::empty({labels.numel()}, opts.dtype(at::kDouble));
   auto stats = at::empty({labels.numel(), 2}, opts);
   auto out = at::empty({count}, opts);
   if (labels.numel())
-    launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), nullptr);
+    launch_stats(logits, labels, ignore, temperature, stats, lp, nullptr);
   if (count)
     by_length(labels.numel(), count, [&](auto block) {
       constexpr int BLOCK = decltype(block)::value;
       hipLaunchKernelGGL((sequence_sum_kernel<BLOCK>), dim3(count), dim3(BLOCK), 0, current_stream(),
-                         lp.data_ptr<float>(), labels.data_ptr<long>(), ignore, seqs, average, out.data_ptr<float>());
+                         lp.data_ptr<double>(), labels.data_ptr<long>(), ignore, seqs, average, out.data_ptr<float>());
     });
   HIP_CHECK(hipGetLastError());
   return {out, stats};
@@ -948,17 +984,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_forward(
   const float* rf = floats(ref, logits, 2 * pairs, "ref_log_probs");
   const long rows = labels.numel();
   auto opts = logits.options().dtype(at::kFloat);
-  auto lp = at::empty({rows}, opts);
+  auto lp = at::empty({rows}, opts.dtype(at::kDouble));
   auto stats = at::empty({rows, 2}, opts);
   auto coef = cu ? at::zeros({rows}, opts) : at::empty({rows}, opts);
   auto rewards = at::empty({2 * pairs}, opts);
   auto loss = at::empty({}, opts);
   auto partial = at::empty({pairs + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
   int* arrived = (int*)(partial.data_ptr<double>() + pairs);
-  launch_stats(logits, labels, ignore, 1.0, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), arrived);
+  launch_stats(logits, labels, ignore, 1.0, stats, lp, arrived);
   by_length(rows, 2 * pairs, [&](auto block) {
     constexpr int BLOCK = decltype(block)::value;
-    hipLaunchKernelGGL((preference_kernel<BLOCK>), dim3(pairs), dim3(BLOCK), 0, current_stream(), lp.data_ptr<float>(),
+    hipLaunchKernelGGL((preference_kernel<BLOCK>), dim3(pairs), dim3(BLOCK), 0, current_stream(), lp.data_ptr<double>(),
                        labels.data_ptr<long>(), ignore, seqs, rf, pairs, (int)kind, beta, smoothing, average,
                        coef.data_ptr<float>(), rewards.data_ptr<float>(), partial.data_ptr<double>(), arrived,
                        loss.data_ptr<float>());
@@ -989,7 +1025,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_fo
   else loss = at::empty({}, opts);
   auto partial = at::empty({2 * count + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
   int* arrived = (int*)(partial.data_ptr<double>() + 2 * count);
-  launch_stats(logits, labels, ignore, temperature, (float2*)stats.data_ptr<float>(), lp.data_ptr<float>(), arrived);
+  launch_stats(logits, labels, ignore, temperature, stats, lp, arrived);
   by_length(rows, count, [&](auto block) {
     constexpr int BLOCK = decltype(block)::value;
     hipLaunchKernelGGL((policy_kernel<BLOCK>), dim3(count), dim3(BLOCK), 0, current_stream(), lp.data_ptr<float>(),
@@ -1028,10 +1064,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
   at::Tensor grad;
   bool held = false;
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "policy_loss", ([&] {
-    const long whole = V / Pack<scalar_t>::width;
-    auto launch = [&](auto block, auto packs) {
-      constexpr int BLOCK = decltype(block)::value, NP = decltype(packs)::value;
-      if (held || whole > BLOCK * NP) return;
+    const long packs = V / Pack<scalar_t>::width;  // one less in rows at odd addresses
+    auto launch = [&](auto block, auto most) {
+      constexpr int BLOCK = decltype(block)::value, NP = decltype(most)::value;
+      if (held || packs > BLOCK * NP) return;
       held = true;
       grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
       const Rows where = rows_of(logits);
@@ -1043,11 +1079,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
                            count, policy, reduction == SEQUENCE, weights, applied.data_ptr<float>(),
                            lp.data_ptr<float>(), losses, (scalar_t*)grad.data_ptr());
     };
-    auto launch_of = [&](auto block, auto... packs) { (launch(block, packs), ...); };
+    auto launch_of = [&](auto block, auto... most) { (launch(block, most), ...); };
     // the fewest lanes that hold a row in up to 16 packs each: there is room for other rows on the compute unit then,
     // which read while this one waits for its sum
     using std::integral_constant;
-    launch_of(integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{},
+    launch_of(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{},
+              integral_constant<int, 6>{}, integral_constant<int, 8>{});
+    launch_of(integral_constant<int, 256>{}, integral_constant<int, 4>{},
               integral_constant<int, 6>{}, integral_constant<int, 8>{}, integral_constant<int, 10>{},
               integral_constant<int, 12>{}, integral_constant<int, 14>{}, integral_constant<int, 16>{});
     launch_of(integral_constant<int, 512>{}, integral_constant<int, 10>{}, integral_constant<int, 12>{},
