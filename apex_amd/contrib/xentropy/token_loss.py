@@ -7,7 +7,8 @@ first training.
 
 All take logits ``[..., V]`` (fp32, fp16 or bf16) and labels of the leading shape: ``labels[i]`` is the token whose
 log-probability row ``i`` of the logits gives, so a causal model's labels are its tokens moved one place to the left.
-Rows whose label is ``ignore_index`` (prompts, padding) are not read and get no gradient, whatever they hold.
+Rows whose label is ``ignore_index`` (prompts, padding) are not read and get no gradient, whatever they hold; rows
+whose gradient turns out to be 0 (clipped tokens) are not read in the backward pass.
 
 On the GPU a loss is one pass over the logits, which keeps two floats of each row, a small pass over the rows'
 log-probabilities, and in the backward pass one more read of the logits while their gradient is written: no
@@ -40,8 +41,8 @@ def _check(logits, labels, ignore_index, temperature=1.0):
         raise ValueError(f"labels must have shape {tuple(logits.shape[:-1])}, got {tuple(labels.shape)}")
     if labels.device != logits.device:
         raise ValueError(f"labels are on {labels.device}, logits on {logits.device}")
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6], got {temperature}")
     return labels.contiguous() if labels.dtype == torch.int64 else labels.long().contiguous()
 
 
@@ -146,7 +147,8 @@ def preference_loss(logits, labels, ref_log_probs, beta=0.1, label_smoothing=0.0
     Args:
         logits: ``[2 * pairs, length, V]``, or with ``cu_seqlens`` ``[tokens, V]``.
         ref_log_probs: ``[2 * pairs]``, as :func:`sequence_log_probs` gives them (with the same ``average``).
-        cu_seqlens: int32 ``[2 * pairs + 1]``, the sequences' first tokens; tokens outside them have no part.
+        cu_seqlens: int32 ``[2 * pairs + 1]``, the sequences' first tokens, which do not fall; tokens outside them have
+            no part.
 
     Returns:
         ``(loss, chosen_rewards, rejected_rewards)``: the loss, differentiable in the logits, and
@@ -174,11 +176,13 @@ def preference_loss(logits, labels, ref_log_probs, beta=0.1, label_smoothing=0.0
     z = beta * (gain[:pairs] - gain[pairs:])
     if loss_type == "sigmoid":
         softplus = torch.nn.functional.softplus
-        loss = (1 - label_smoothing) * softplus(-z, threshold=1e9) + label_smoothing * softplus(z, threshold=1e9)
+        loss = (1 - label_smoothing) * softplus(-z, threshold=1e9)
+        if label_smoothing:
+            loss = loss + label_smoothing * softplus(z, threshold=1e9)
     elif loss_type == "ipo":
         loss = (z / beta - 0.5 / beta) ** 2
     else:
-        loss = torch.where(z >= 1, 0.0 * z, 1 - z)
+        loss = torch.where(z >= 1, 0.0, 1 - z)
     rewards = (beta * gain).detach().float()
     return loss.mean().float(), rewards[:pairs], rewards[pairs:]
 

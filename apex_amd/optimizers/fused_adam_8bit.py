@@ -125,6 +125,9 @@ class FusedAdam8bit(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         # torch casts state to the params' type: the codes and scales are put back as they were saved
         saved = state_dict["state"]
+        for state in saved.values():
+            if state and not all(k in state for k in _STATE):
+                raise ValueError(f"FusedAdam8bit needs the state {_STATE} for each param, got {tuple(state)}")
         super().load_state_dict(state_dict)
         order = [k for g in state_dict["param_groups"] for k in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]

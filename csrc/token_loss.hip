@@ -9,7 +9,8 @@
 // lp that makes the loss and c, and a backward pass that reads the logits again
 // and writes their gradient. Rows whose label is `ignore` are not read; their lp
 // is 0 and their gradient rows are 0. A label outside [0, V) reads nothing and
-// gives NaN.
+// gives NaN. Rows whose gradient is 0 (a clipped token, a weight of 0) are not
+// read in the backward pass either.
 //
 // What bounds them: HBM. Forward reads the labelled rows once, backward reads
 // them once more and writes the whole gradient.
@@ -49,7 +50,7 @@ struct Sequences {
   }
 };
 
-// The sequence of a row, -1 where none has it
+// The sequence of a row, -1 where none has it (cu does not fall)
 __device__ __forceinline__ long owner_of(const Sequences& seqs, long count, long row) {
   if (!seqs.cu) return row / seqs.length;
   long lo = 0, hi = count - 1;  // the last one that begins at or before the row
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(BLOCK) preference_kernel(
     const double e = exp(-fabs(z)), soft = log1p(e);
     const double minus = fmax(-z, 0.0) + soft, plus = fmax(z, 0.0) + soft;
     const double up = (z >= 0 ? e : 1.0) / (1.0 + e);  // sigmoid(-z)
-    loss = (1.0 - smoothing) * minus + smoothing * plus;
+    loss = (1.0 - smoothing) * minus + (smoothing > 0 ? smoothing * plus : 0.0);  // plus may be infinite
     slope = beta * (smoothing * (1.0 - up) - (1.0 - smoothing) * up);
   } else if (kind == IPO) {
     const double off = d - 0.5 / beta;

@@ -181,6 +181,14 @@ def test_a_checkpoint_goes_on_bit_for_bit(master):
 
 
 def test_refusals():
+    from apex_amd.optimizers import FusedAdam
+
+    w = torch.nn.Parameter(torch.zeros(3))
+    w.grad = torch.ones(3)
+    other = FusedAdam([w])
+    other.step()
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        FusedAdam8bit([w]).load_state_dict(other.state_dict())
     p = torch.nn.Parameter(torch.zeros(3))
     with pytest.raises(RuntimeError, match="AMSGrad"):
         FusedAdam8bit([p], amsgrad=True)

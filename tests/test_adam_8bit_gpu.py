@@ -196,6 +196,33 @@ def test_layouts():
     torch.testing.assert_close(out[0].cpu(), q.detach(), rtol=0, atol=4 * 2 ** -24 * 5)
 
 
+def test_a_tensor_beyond_32_bits():
+    """2^31 + 131 elements: those behind 2^31 are stepped as a small tensor's are, but for their random numbers."""
+    n, tail = 2 ** 31 + 131, 131
+    g = torch.Generator().manual_seed(3)
+    w, d = torch.randn(tail, generator=g), torch.randn(tail, generator=g)
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    p.detach()[-tail:] = w.cuda()
+    p.grad[-tail:] = d.cuda()
+    opt = FusedAdam8bit([p], lr=1e-2)
+    opt.step()
+    q = torch.nn.Parameter(w.bfloat16())
+    q.grad = d.bfloat16()
+    small = FusedAdam8bit([q], lr=1e-2)
+    small.step()
+    # rounded to bf16, and where fp32 differs in its last bits to the other side
+    torch.testing.assert_close(p.detach()[-tail:].cpu(), q.detach(), rtol=2 ** -7, atol=0)
+    for k in ("exp_avg", "exp_avg_sq"):
+        s, t = opt.state[p], small.state[q]
+        torch.testing.assert_close(s[k + "_scale"][-2:].cpu(), t[k + "_scale"], rtol=8 * 2 ** -24, atol=0)
+        # of the two codes around a value each takes one: at most a code's distance, 1/8 of the larger or 2^-9, apart
+        a, b = s[k][-tail:].cpu().float(), t[k].float()
+        assert ((a - b).abs() <= torch.maximum(torch.maximum(a.abs(), b.abs()) / 8, torch.tensor(2.0 ** -9))).all()
+        assert not s[k].view(torch.uint8)[:-tail].any()
+    assert not p.detach()[:-tail].any()
+
+
 def test_infinite_and_nan_gradients_stay_where_they_are():
     for dtype in (torch.float32, torch.bfloat16):
         p = torch.nn.Parameter(torch.ones(1000, device="cuda", dtype=dtype))

@@ -107,6 +107,19 @@ def test_policy_loss(reduction, cu, by_row, kl, on_policy):
     torch.testing.assert_close(b, a, **TOL)
 
 
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge"])
+def test_a_rejected_answer_that_cannot_be(kind):
+    """A rejected token of probability 0: the pair is as right as can be, and asks for nothing."""
+    x = torch.zeros(2, 3, 5)
+    x[1, 1, 4] = -math.inf
+    y = torch.tensor([[0, 1, 2], [3, 4, 0]])
+    x.requires_grad_(True)
+    loss, _, rejected = preference_loss(x, y, torch.zeros(2), loss_type=kind)
+    assert loss == 0 and rejected[0] == -math.inf
+    loss.backward()
+    assert (x.grad == 0).all()
+
+
 def test_gradients_against_differences():
     """The formulas' gradients, in 64 bits, against central differences: what the other tests hold the kernels to."""
     x, y, g = make((4, 3), 6)
@@ -129,7 +142,7 @@ def test_refusals():
         token_log_probs(x, y[:, :4])
     with pytest.raises(ValueError, match="vocabulary"):
         token_log_probs(x[..., :0], y)
-    for t in (0.0, -1.0, math.inf, math.nan):
+    for t in (0.0, -1.0, 1e-7, 1e7, math.inf, math.nan):
         with pytest.raises(ValueError, match="temperature"):
             token_log_probs(x, y, temperature=t)
     with pytest.raises(ValueError, match="cu_seqlens"):

@@ -226,6 +226,61 @@ def test_preference_far_out(kind, shift):
     near(dx, want, oracle.grad_bound(x, y, torch.full(y.shape, 0.1), torch.float32))
 
 
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge"])
+def test_a_rejected_answer_that_cannot_be(kind):
+    """A rejected token of probability 0: the pair is as right as can be, and asks for nothing."""
+    x = torch.zeros(2, 3, 5, device="cuda")
+    x[1, 1, 4] = -math.inf
+    y = torch.tensor([[0, 1, 2], [3, 4, 0]], device="cuda")
+    x.requires_grad_(True)
+    loss, _, rejected = preference_loss(x, y, torch.zeros(2, device="cuda"), loss_type=kind)
+    assert loss == 0 and rejected[0] == -math.inf
+    loss.backward()
+    assert (x.grad == 0).all()
+
+
+def test_nothing_is_labelled():
+    """Whole batches of padding: losses of 0 (or of the references alone), gradients of 0."""
+    x = torch.full((4, 3, 9), math.nan, device="cuda", requires_grad=True)
+    y = torch.full((4, 3), -100, device="cuda")
+    adv = torch.ones(4, device="cuda")
+    for reduction in ("token", "sequence", "sum"):
+        for scale in (None, 1.0):
+            loss, lp = policy_loss(x, y, None, adv, reduction=reduction, grad_scale=scale)
+            assert loss == 0 and (lp == 0).all()
+            assert (grad_of(loss, x, torch.tensor(1.0)) == 0).all()
+    loss, chosen, _ = preference_loss(x, y, adv, average=True)
+    assert abs(float(loss.detach()) - math.log(2)) < 1e-6 and (chosen == -0.1 * adv[:2]).all()
+    assert (grad_of(loss, x, torch.tensor(1.0)) == 0).all()
+    assert (sequence_log_probs(x, y, average=True) == 0).all()
+
+
+def test_one_token():
+    x, y, _ = make((1, 1), 32000, torch.bfloat16, ignored=0)
+    got = token_log_probs(x.cuda(), y.cuda())
+    near(got, oracle.log_probs(x.double(), y), oracle.lp_bound(x, y))
+    assert torch.equal(sequence_log_probs(x.cuda(), y.cuda()), got.view(1))
+    flat = policy_loss(x.cuda().view(1, 32000), y.cuda().view(1), None, torch.ones(1, device="cuda"))[0]
+    assert flat.item() == -1.0
+
+
+def test_many_rows_of_a_small_vocabulary():
+    """More rows than a grid has blocks along one side, more sequences than a block has threads."""
+    x, y, g = make((70000,), 6, torch.float32)
+    cu = torch.arange(0, 70001, 7, dtype=torch.int32)
+    x64, xg = x.double().requires_grad_(True), x.cuda().requires_grad_(True)
+    lp = oracle.log_probs(x64, y)
+    got = sequence_log_probs(xg, y.cuda(), cu.cuda())
+    near(got, lp.view(-1, 7).sum(1), oracle.lp_bound(x, y).view(-1, 7).sum(1) + U * 100)
+    near(grad_of(got, xg, torch.ones(10000)), torch.autograd.grad(lp.sum(), x64)[0], oracle.grad_bound(x, y, torch.ones(70000), torch.float32))
+    adv = torch.randn(10000, generator=g)
+    want, _ = oracle.policy(x.double(), y, None, adv, reduction="sequence", cu=cu.tolist())
+    for scale in (None, 1.0):
+        loss, _ = policy_loss(xg, y.cuda(), None, adv.cuda(), reduction="sequence", cu_seqlens=cu.cuda(), grad_scale=scale)
+        # 10^4 means of -A, each rounded a few times; their sum in 64 bits
+        near(loss, want, 4 * U * adv.abs().mean().double())
+
+
 def policy_case(packed, dtype, vocab, by_row, kl, on_policy, temperature, seed=0):
     x, y, g, cu, cug = layout_of(packed, vocab, dtype)
     lp = oracle.log_probs(x.double(), y, temperature=temperature).float()
@@ -466,3 +521,28 @@ def test_gradients_add_up_over_calls():
     want = torch.autograd.grad(preference_loss(b, y.cuda(), ref)[0], b)[0] + torch.autograd.grad(policy_loss(b, y.cuda(), None, ref + 1)[0], b)[0]
     # fp32 sums of two values under 1, each within some half steps
     torch.testing.assert_close(a.grad, want, rtol=0, atol=8 * 2 ** -24)
+
+
+def test_rows_beyond_32_bits():
+    """Rows that begin, and gradients that lie, more than 2^31 elements from the first."""
+    g = torch.Generator().manual_seed(0)
+    few = torch.randn(2, 300, generator=g)
+    base = torch.empty(2_200_000_300, dtype=torch.bfloat16, device="cuda")
+    x = base.as_strided((2, 300), (2_200_000_000, 1))
+    x.copy_(few)
+    y = torch.tensor([3, 299])
+    few = few.to(torch.bfloat16)
+    near(token_log_probs(x, y.cuda()), oracle.log_probs(few.double(), y), oracle.lp_bound(few, y))
+    del base, x
+    rows, vocab = 70000, 32000
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    last = (torch.randn(2, vocab, generator=g) * 2).to(torch.bfloat16)
+    x[-2:] = last.cuda()
+    y = torch.full((rows,), -100, device="cuda")
+    y[-2:] = torch.tensor([5, 31999], device="cuda")
+    x.requires_grad_(True)
+    dx = grad_of(token_log_probs(x, y), x, torch.ones(rows))
+    l64 = last.double().requires_grad_(True)
+    lp = oracle.log_probs(l64, y[-2:].cpu())
+    near(dx[-2:], torch.autograd.grad(lp.sum(), l64)[0], oracle.grad_bound(last, y[-2:].cpu(), torch.ones(2), torch.bfloat16))
+    assert not dx[:-2].any()
