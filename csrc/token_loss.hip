@@ -491,8 +491,8 @@ template <int BLOCK>
 __global__ void __launch_bounds__(BLOCK) preference_kernel(
     const double* __restrict__ lp, const long* __restrict__ labels, long ignore, Sequences seqs,
     const float* __restrict__ ref, long pairs, int kind, double beta, double smoothing, bool average,
-    float* __restrict__ coef, float* __restrict__ rewards, double* __restrict__ partial,
-    int* __restrict__ arrived, float* __restrict__ loss_out) {
+    float* __restrict__ coef, float* __restrict__ chosen_out, float* __restrict__ rejected_out,
+    double* __restrict__ partial, int* __restrict__ arrived, float* __restrict__ loss_out) {
   __shared__ double smem[4 * BLOCK / WAVE_SIZE];
   __shared__ int last;
   const long b = blockIdx.x;
@@ -533,8 +533,8 @@ __global__ void __launch_bounds__(BLOCK) preference_kernel(
     for (long r = begin[k] + threadIdx.x; r < end[k]; r += BLOCK) coef[r] = f;
   }
   if (threadIdx.x == 0) {
-    rewards[b] = (float)(beta * chosen);
-    rewards[b + pairs] = (float)(beta * rejected);
+    chosen_out[b] = (float)(beta * chosen);
+    rejected_out[b] = (float)(beta * rejected);
     partial[b] = loss;
   }
   if (!comes_last(arrived, gridDim.x, &last)) return;
@@ -838,11 +838,25 @@ Policy policy_of(const at::Tensor& logits, const c10::optional<at::Tensor>& old,
           floats(advantages, logits, by_row ? rows : count, "advantages"), by_row, (float)low, (float)high, (float)kl};
 }
 
+// What the backward pass of a loss needs, in one allocation: of each row its
+// statistics and its coefficient, and the number that all coefficients are
+// multiplied by.
+struct Kept {
+  at::Tensor room;
+  float *stats, *coef, *norm;
+  static Kept of(const at::Tensor& room, long rows) {
+    float* p = room.data_ptr<float>();
+    return {room, p, p + 2 * rows, p + 3 * rows};
+  }
+  // rows behind the last packed sequence belong to none: no loss, no gradient
+  static Kept make(const at::TensorOptions& opts, long rows, bool packed) {
+    return of(packed ? at::zeros({3 * rows + 1}, opts) : at::empty({3 * rows + 1}, opts), rows);
+  }
+};
+
 void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, double temperature,
-                  const at::Tensor& stats, const at::Tensor& lp, int* arrived) {
-  const bool wide = lp.scalar_type() == at::kDouble;
-  const RowOut out{(float2*)stats.data_ptr<float>(), wide ? nullptr : lp.data_ptr<float>(),
-                   wide ? lp.data_ptr<double>() : nullptr};
+                  float* stats, float* lp, double* lp64, int* arrived) {
+  const RowOut out{(float2*)stats, lp, lp64};
   const Rows where = rows_of(logits);
   const long V = logits.size(-1), rows = labels.numel();
   const Base c = base_of(temperature);
@@ -898,24 +912,21 @@ std::tuple<at::Tensor, at::Tensor> token_forward(at::Tensor logits, at::Tensor l
   auto lp = at::empty(labels.sizes(), opts);
   auto stats = at::empty({labels.numel(), 2}, opts);
   if (labels.numel())
-    launch_stats(logits, labels, ignore, temperature, stats, lp, nullptr);
+    launch_stats(logits, labels, ignore, temperature, stats.data_ptr<float>(), lp.data_ptr<float>(), nullptr, nullptr);
   return {lp, stats};
 }
 
-at::Tensor rows_backward(at::Tensor logits, at::Tensor labels, at::Tensor stats, at::Tensor coef,
-                         c10::optional<at::Tensor> scale, c10::optional<at::Tensor> norm, long ignore,
-                         double temperature) {
+// The logits' gradient from that of the rows' log-probabilities: coef, times `scale` (one value, or one a row) and `norm`
+at::Tensor rows_backward(at::Tensor logits, const at::Tensor& labels, const float* stats, const float* coef,
+                         const at::Tensor& scale, const float* norm, long ignore, double temperature) {
   check_rows(logits, labels);
   const at::DeviceGuard guard(logits.device());
   const long rows = labels.numel(), V = logits.size(-1);
   auto grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
   if (!rows) return grad;
   const Rows where = rows_of(logits);
-  const float* st = floats(stats, logits, 2 * rows, "stats");
-  const float* co = floats(coef, logits, rows, "coef");
-  const float* sc = scale ? floats(*scale, logits, scale->numel() == 1 ? 1 : rows, "grad_output") : nullptr;
-  const float* no = norm ? floats(*norm, logits, 1, "norm") : nullptr;
-  const long step = scale && scale->numel() == rows && rows > 1 ? 1 : 0;
+  const float* sc = scale.defined() ? floats(scale, logits, scale.numel() == 1 ? 1 : rows, "grad_output") : nullptr;
+  const long step = scale.defined() && scale.numel() == rows && rows > 1 ? 1 : 0;
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
     const long lanes = std::max(V / Pack<scalar_t>::width, 1L);
     auto launch = [&](auto block) {
@@ -924,7 +935,7 @@ at::Tensor rows_backward(at::Tensor logits, at::Tensor labels, at::Tensor stats,
       hipLaunchKernelGGL((row_grad_kernel<scalar_t, BLOCK>), grid, dim3(BLOCK), 0, current_stream(),
                          (const scalar_t*)logits.data_ptr(), where, labels.data_ptr<long>(), ignore, V, rows,
                          (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature),
-                         (const float2*)st, co, sc, step, no, (scalar_t*)grad.data_ptr());
+                         (const float2*)stats, coef, sc, step, norm, (scalar_t*)grad.data_ptr());
     };
     if (lanes <= 64) launch(std::integral_constant<int, 64>{});
     else if (lanes <= 128) launch(std::integral_constant<int, 128>{});
@@ -946,7 +957,7 @@ std::tuple<at::Tensor, at::Tensor> sequence_forward(at::Tensor logits, at::Tenso
   auto stats = at::empty({labels.numel(), 2}, opts);
   auto out = at::empty({count}, opts);
   if (labels.numel())
-    launch_stats(logits, labels, ignore, temperature, stats, lp, nullptr);
+    launch_stats(logits, labels, ignore, temperature, stats.data_ptr<float>(), nullptr, lp.data_ptr<double>(), nullptr);
   if (count)
     by_length(labels.numel(), count, [&](auto block) {
       constexpr int BLOCK = decltype(block)::value;
@@ -974,10 +985,10 @@ at::Tensor sequence_coef(at::Tensor grad, at::Tensor labels, c10::optional<at::T
   return coef;
 }
 
-// -> (loss, rewards [2 pairs], stats, coef)
+// -> (loss, chosen rewards, rejected rewards, kept)
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_forward(
-    at::Tensor logits, at::Tensor labels, at::Tensor ref, c10::optional<at::Tensor> cu, long pairs, long kind,
-    double beta, double smoothing, bool average, long ignore) {
+    const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ref, const c10::optional<at::Tensor>& cu,
+    long pairs, long kind, double beta, double smoothing, bool average, long ignore) {
   check_rows(logits, labels);
   const at::DeviceGuard guard(logits.device());
   TORCH_CHECK(labels.numel() > 0 && pairs > 0, "preference_loss: needs a pair and a row");
@@ -985,30 +996,29 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_forward(
   const float* rf = floats(ref, logits, 2 * pairs, "ref_log_probs");
   const long rows = labels.numel();
   auto opts = logits.options().dtype(at::kFloat);
-  auto lp = at::empty({rows}, opts.dtype(at::kDouble));
-  auto stats = at::empty({rows, 2}, opts);
-  auto coef = cu ? at::zeros({rows}, opts) : at::empty({rows}, opts);
-  auto rewards = at::empty({2 * pairs}, opts);
-  auto loss = at::empty({}, opts);
-  auto partial = at::empty({pairs + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
-  int* arrived = (int*)(partial.data_ptr<double>() + pairs);
-  launch_stats(logits, labels, ignore, 1.0, stats, lp, arrived);
+  const Kept kept = Kept::make(opts, rows, cu.has_value());
+  auto chosen = at::empty({pairs}, opts), rejected = at::empty({pairs}, opts), loss = at::empty({}, opts);
+  auto room = at::empty({rows + pairs + 1}, opts.dtype(at::kDouble));  // log-probabilities, the pairs' losses, the counter
+  double *lp = room.data_ptr<double>(), *partial = lp + rows;
+  int* arrived = (int*)(partial + pairs);
+  launch_stats(logits, labels, ignore, 1.0, kept.stats, nullptr, lp, arrived);
   by_length(rows, 2 * pairs, [&](auto block) {
     constexpr int BLOCK = decltype(block)::value;
-    hipLaunchKernelGGL((preference_kernel<BLOCK>), dim3(pairs), dim3(BLOCK), 0, current_stream(), lp.data_ptr<double>(),
+    hipLaunchKernelGGL((preference_kernel<BLOCK>), dim3(pairs), dim3(BLOCK), 0, current_stream(), lp,
                        labels.data_ptr<long>(), ignore, seqs, rf, pairs, (int)kind, beta, smoothing, average,
-                       coef.data_ptr<float>(), rewards.data_ptr<float>(), partial.data_ptr<double>(), arrived,
+                       kept.coef, chosen.data_ptr<float>(), rejected.data_ptr<float>(), partial, arrived,
                        loss.data_ptr<float>());
   });
   HIP_CHECK(hipGetLastError());
-  return {loss, rewards, stats, coef};
+  return {loss, chosen, rejected, kept.room};
 }
 
-// -> (loss, lp, stats, coef, norm)
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_forward(
-    at::Tensor logits, at::Tensor labels, c10::optional<at::Tensor> old, at::Tensor advantages,
-    bool by_row, c10::optional<at::Tensor> ref, c10::optional<at::Tensor> cu, long count, double low, double high,
-    double kl, double temperature, long reduction, long ignore) {
+// -> (loss, lp, kept)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> policy_forward(
+    const at::Tensor& logits, const at::Tensor& labels, const c10::optional<at::Tensor>& old,
+    const at::Tensor& advantages, bool by_row, const c10::optional<at::Tensor>& ref,
+    const c10::optional<at::Tensor>& cu, long count, double low, double high, double kl, double temperature,
+    long reduction, long ignore) {
   check_rows(logits, labels);
   const at::DeviceGuard guard(logits.device());
   const long rows = labels.numel();
@@ -1016,33 +1026,31 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_fo
   const Sequences seqs = sequences_of(labels, cu, count);
   const Policy policy = policy_of(logits, old, advantages, by_row, ref, rows, count, low, high, kl);
   auto opts = logits.options().dtype(at::kFloat);
+  const Kept kept = Kept::make(opts, rows, cu.has_value());
   auto lp = at::empty(labels.sizes(), opts);
-  auto stats = at::empty({rows, 2}, opts);
-  // rows behind the last packed sequence belong to none: no loss, no gradient
-  auto coef = cu ? at::zeros({rows}, opts) : at::empty({rows}, opts);
-  auto norm = at::empty({1}, opts);
   at::Tensor loss;
   if (reduction == NONE) loss = cu ? at::zeros(labels.sizes(), opts) : at::empty(labels.sizes(), opts);
   else loss = at::empty({}, opts);
-  auto partial = at::empty({2 * count + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
-  int* arrived = (int*)(partial.data_ptr<double>() + 2 * count);
-  launch_stats(logits, labels, ignore, temperature, stats, lp, arrived);
+  auto room = at::empty({2 * count + 1}, opts.dtype(at::kDouble));  // the sequences' losses and tokens, the counter
+  double* partial = room.data_ptr<double>();
+  int* arrived = (int*)(partial + 2 * count);
+  launch_stats(logits, labels, ignore, temperature, kept.stats, lp.data_ptr<float>(), nullptr, arrived);
   by_length(rows, count, [&](auto block) {
     constexpr int BLOCK = decltype(block)::value;
     hipLaunchKernelGGL((policy_kernel<BLOCK>), dim3(count), dim3(BLOCK), 0, current_stream(), lp.data_ptr<float>(),
-                       labels.data_ptr<long>(), ignore, seqs, policy, (int)reduction, coef.data_ptr<float>(),
-                       loss.data_ptr<float>(), partial.data_ptr<double>(), arrived, norm.data_ptr<float>(),
-                       loss.data_ptr<float>());
+                       labels.data_ptr<long>(), ignore, seqs, policy, (int)reduction, kept.coef,
+                       loss.data_ptr<float>(), partial, arrived, kept.norm, loss.data_ptr<float>());
   });
   HIP_CHECK(hipGetLastError());
-  return {loss, lp, stats, coef, norm};
+  return {loss, lp, kept.room};
 }
 
 // The gradient is made here, for a gradient of the loss that is known -> (loss, lp, dlogits, applied)
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
-    at::Tensor logits, at::Tensor labels, c10::optional<at::Tensor> old, at::Tensor advantages, bool by_row,
-    c10::optional<at::Tensor> ref, c10::optional<at::Tensor> cu, long count, double low, double high, double kl,
-    double temperature, long reduction, long ignore, double scale, c10::optional<at::Tensor> scale_tensor) {
+    at::Tensor logits, const at::Tensor& labels, const c10::optional<at::Tensor>& old, const at::Tensor& advantages,
+    bool by_row, const c10::optional<at::Tensor>& ref, const c10::optional<at::Tensor>& cu, long count, double low,
+    double high, double kl, double temperature, long reduction, long ignore, double scale,
+    const c10::optional<at::Tensor>& scale_tensor) {
   check_rows(logits, labels);
   const at::DeviceGuard guard(logits.device());
   const long rows = labels.numel(), V = logits.size(-1);
@@ -1053,32 +1061,34 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
   const Policy policy = policy_of(logits, old, advantages, by_row, ref, rows, count, low, high, kl);
   const float* value = scale_tensor ? floats(*scale_tensor, logits, 1, "grad_scale") : nullptr;
   const long groups = reduction == SEQUENCE ? count : 1;
-  auto loss = at::empty({}, opts), lp = at::empty(labels.sizes(), opts), applied = at::empty({1}, opts);
-  auto room = at::empty({groups + rows}, opts);  // weights, and the rows' losses
-  auto partial = at::empty({64 + 1}, opts.dtype(at::kDouble));  // the last one holds the counter
-  int* arrived = (int*)(partial.data_ptr<double>() + 64);
-  float *weights = room.data_ptr<float>(), *losses = weights + groups;
+  const long blocks = std::min<long>(64, (rows + 4 * TOTAL_BLOCK - 1) / (4 * TOTAL_BLOCK));
+  // blocks' sums in 64 bits, what the gradient is multiplied by, a counter, the weights, and the rows' losses
+  auto room = at::empty({2 * blocks + 2 + groups + rows}, opts);
+  auto* partial = (double*)room.data_ptr<float>();
+  auto applied = room.narrow(0, 2 * blocks, 1);
+  float *ap = (float*)(partial + blocks), *weights = ap + 2, *losses = weights + groups;
+  int* arrived = (int*)(ap + 1);
   hipLaunchKernelGGL(policy_prepare_kernel, dim3(groups), dim3(PREPARE_BLOCK), 0, current_stream(),
-                     labels.data_ptr<long>(), ignore, seqs, count, (int)reduction, (float)scale, value,
-                     applied.data_ptr<float>(), weights, arrived);
+                     labels.data_ptr<long>(), ignore, seqs, count, (int)reduction, (float)scale, value, ap, weights,
+                     arrived);
   HIP_CHECK(hipGetLastError());
-  at::Tensor grad;
-  bool held = false;
+  at::Tensor grad, loss, lp;
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "policy_loss", ([&] {
     const long packs = V / Pack<scalar_t>::width;  // one less in rows at odd addresses
     auto launch = [&](auto block, auto most) {
       constexpr int BLOCK = decltype(block)::value, NP = decltype(most)::value;
-      if (held || packs > BLOCK * NP) return;
-      held = true;
+      if (grad.defined() || packs > BLOCK * NP) return;
       grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+      loss = at::empty({}, opts);
+      lp = at::empty(labels.sizes(), opts);
       const Rows where = rows_of(logits);
       constexpr long MOST = 1 << 20;  // a launch's threads are counted in 32 bits
       for (long first = 0; first < rows; first += MOST)
         hipLaunchKernelGGL((policy_at_once_kernel<scalar_t, BLOCK, NP>), dim3(std::min(MOST, rows - first)),
                            dim3(BLOCK), 0, current_stream(), (const scalar_t*)logits.data_ptr(), where,
                            labels.data_ptr<long>(), ignore, V, first, base_of(temperature), 1.0 / temperature, seqs,
-                           count, policy, reduction == SEQUENCE, weights, applied.data_ptr<float>(),
-                           lp.data_ptr<float>(), losses, (scalar_t*)grad.data_ptr());
+                           count, policy, reduction == SEQUENCE, weights, ap, lp.data_ptr<float>(), losses,
+                           (scalar_t*)grad.data_ptr());
     };
     auto launch_of = [&](auto block, auto... most) { (launch(block, most), ...); };
     // the fewest lanes that hold a row in up to 16 packs each: there is room for other rows on the compute unit then,
@@ -1095,14 +1105,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_at_once(
               integral_constant<int, 14>{}, integral_constant<int, 16>{});
   }()));
   HIP_CHECK(hipGetLastError());
-  if (!held) {  // a longer row is read twice
-    auto [loss2, lp2, stats, coef, norm] = policy_forward(logits, labels, old, advantages, by_row, ref, cu, count, low,
-                                                          high, kl, temperature, reduction, ignore);
-    return {loss2, lp2, rows_backward(logits, labels, stats, coef, applied, norm, ignore, temperature), applied};
+  if (!grad.defined()) {  // a longer row is read twice
+    auto [loss2, lp2, room2] = policy_forward(logits, labels, old, advantages, by_row, ref, cu, count, low, high, kl,
+                                              temperature, reduction, ignore);
+    const Kept kept = Kept::of(room2, rows);
+    return {loss2, lp2, rows_backward(logits, labels, kept.stats, kept.coef, applied, kept.norm, ignore, temperature),
+            applied};
   }
-  const long blocks = std::min<long>(64, (rows + 4 * TOTAL_BLOCK - 1) / (4 * TOTAL_BLOCK));
-  hipLaunchKernelGGL(total_kernel, dim3(blocks), dim3(TOTAL_BLOCK), 0, current_stream(), losses, rows,
-                     partial.data_ptr<double>(), arrived, loss.data_ptr<float>());
+  hipLaunchKernelGGL(total_kernel, dim3(blocks), dim3(TOTAL_BLOCK), 0, current_stream(), losses, rows, partial, arrived,
+                     loss.data_ptr<float>());
   HIP_CHECK(hipGetLastError());
   return {loss, lp, grad, applied};
 }
@@ -1134,10 +1145,10 @@ at::Tensor once(const char* name, at::Tensor grad) {
   return (*error)({grad})[0];
 }
 
-// What the gradient of the rows' log-probabilities becomes: kept between the passes
-void keep(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& stats,
-          const at::Tensor& coef, const at::Tensor& norm, long ignore, double temperature) {
-  ctx->save_for_backward({logits, labels, stats, coef, norm});
+// What is kept between the passes; `room` is a Kept's, or the rows' statistics alone
+void keep(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& room, long ignore,
+          double temperature) {
+  ctx->save_for_backward({logits, labels, room});
   ctx->saved_data["ignore"] = (int64_t)ignore;
   ctx->saved_data["temperature"] = temperature;
   ctx->set_materialize_grads(false);
@@ -1149,14 +1160,15 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, int64_t ignore,
                             double temperature) {
     auto [lp, stats] = token_forward(logits, labels, ignore, temperature);
-    keep(ctx, logits, labels, stats, {}, {}, ignore, temperature);
+    keep(ctx, logits, labels, stats, ignore, temperature);
     return lp;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}, {}};
     const auto saved = ctx->get_saved_variables();
-    auto grad = rows_backward(saved[0], saved[1], saved[2], fp32(grads[0].detach()), {}, {},
-                              ctx->saved_data["ignore"].toInt(), ctx->saved_data["temperature"].toDouble());
+    const auto coef = fp32(grads[0].detach());
+    auto grad = rows_backward(saved[0], saved[1], saved[2].data_ptr<float>(), floats(coef, saved[0], saved[1].numel(), "grad_output"),
+                              {}, nullptr, ctx->saved_data["ignore"].toInt(), ctx->saved_data["temperature"].toDouble());
     return {once("token_log_probs", grad), {}, {}, {}};
   }
 };
@@ -1166,7 +1178,8 @@ struct SequenceLogProbs : torch::autograd::Function<SequenceLogProbs> {
                             const c10::optional<at::Tensor>& cu, int64_t count, bool average, int64_t ignore,
                             double temperature) {
     auto [sums, stats] = sequence_forward(logits, labels, cu, count, average, ignore, temperature);
-    keep(ctx, logits, labels, stats, cu ? *cu : at::Tensor(), {}, ignore, temperature);
+    keep(ctx, logits, labels, stats, ignore, temperature);
+    ctx->save_for_backward({logits, labels, stats, cu ? *cu : at::Tensor()});
     ctx->saved_data["average"] = average;
     return sums;
   }
@@ -1176,17 +1189,19 @@ struct SequenceLogProbs : torch::autograd::Function<SequenceLogProbs> {
     const long ignore = ctx->saved_data["ignore"].toInt();
     const auto cu = saved[3].defined() ? c10::optional<at::Tensor>(saved[3]) : c10::nullopt;
     auto coef = sequence_coef(fp32(grads[0].detach()), saved[1], cu, ctx->saved_data["average"].toBool(), ignore);
-    auto grad = rows_backward(saved[0], saved[1], saved[2], coef, {}, {}, ignore, ctx->saved_data["temperature"].toDouble());
+    auto grad = rows_backward(saved[0], saved[1], saved[2].data_ptr<float>(), coef.data_ptr<float>(), {}, nullptr, ignore,
+                              ctx->saved_data["temperature"].toDouble());
     return {once("sequence_log_probs", grad), {}, {}, {}, {}, {}, {}};
   }
 };
 
 // The backward pass of a loss whose coefficients the forward pass has made
-at::Tensor loss_backward(const char* name, AutogradContext* ctx, const at::Tensor& given) {
+at::Tensor loss_backward(const char* name, AutogradContext* ctx, const at::Tensor& given, bool with_norm) {
   const auto saved = ctx->get_saved_variables();
-  const auto norm = saved[4].defined() ? c10::optional<at::Tensor>(saved[4]) : c10::nullopt;
-  return once(name, rows_backward(saved[0], saved[1], saved[2], saved[3], fp32(given.detach()), norm,
-                                  ctx->saved_data["ignore"].toInt(), ctx->saved_data["temperature"].toDouble()));
+  const Kept kept = Kept::of(saved[2], saved[1].numel());
+  return once(name, rows_backward(saved[0], saved[1], kept.stats, kept.coef, fp32(given.detach()),
+                                  with_norm ? kept.norm : nullptr, ctx->saved_data["ignore"].toInt(),
+                                  ctx->saved_data["temperature"].toDouble()));
 }
 
 struct PreferenceCall {
@@ -1200,16 +1215,15 @@ struct PreferenceCall {
 
 struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const PreferenceCall& a) {
-    auto [loss, rewards, stats, coef] = preference_forward(logits, a.labels, a.ref, a.cu, a.pairs, a.kind, a.beta,
-                                                           a.smoothing, a.average, a.ignore);
-    keep(ctx, logits, a.labels, stats, coef, {}, a.ignore, 1.0);
-    auto chosen = rewards.narrow(0, 0, a.pairs), rejected = rewards.narrow(0, a.pairs, a.pairs);
+    auto [loss, chosen, rejected, room] = preference_forward(logits, a.labels, a.ref, a.cu, a.pairs, a.kind, a.beta,
+                                                             a.smoothing, a.average, a.ignore);
+    keep(ctx, logits, a.labels, room, a.ignore, 1.0);
     ctx->mark_non_differentiable({chosen, rejected});
     return {loss, chosen, rejected};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}};
-    return {loss_backward("preference_loss", ctx, grads[0]), {}};
+    return {loss_backward("preference_loss", ctx, grads[0], false), {}};
   }
 };
 
@@ -1223,15 +1237,16 @@ struct PolicyCall {
 
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const PolicyCall& a) {
-    auto [loss, lp, stats, coef, norm] = policy_forward(logits, a.labels, a.old, a.advantages, a.by_row, a.ref, a.cu,
-                                                        a.count, a.low, a.high, a.kl, a.temperature, a.reduction, a.ignore);
-    keep(ctx, logits, a.labels, stats, coef, a.reduction == TOKEN ? norm : at::Tensor(), a.ignore, a.temperature);
+    auto [loss, lp, room] = policy_forward(logits, a.labels, a.old, a.advantages, a.by_row, a.ref, a.cu, a.count, a.low,
+                                           a.high, a.kl, a.temperature, a.reduction, a.ignore);
+    keep(ctx, logits, a.labels, room, a.ignore, a.temperature);
+    ctx->saved_data["norm"] = a.reduction == TOKEN;
     ctx->mark_non_differentiable({lp});
     return {loss, lp};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}};
-    return {loss_backward("policy_loss", ctx, grads[0]), {}};
+    return {loss_backward("policy_loss", ctx, grads[0], ctx->saved_data["norm"].toBool()), {}};
   }
 };
 
