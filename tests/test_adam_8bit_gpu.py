@@ -391,3 +391,35 @@ def test_a_post_training_step_of_all_of_them():
             opt.step()
             for p, b in zip(model.parameters(), before):
                 assert torch.isfinite(p).all() and (p.numel() < 1000 or not torch.equal(p, b))
+
+
+@pytest.mark.parametrize("level", ["O1", "O2"])
+def test_under_amp(level):
+    """amp's own masters (O2) and its loss scale. The first step is FusedAdam's, for it is made of moments that have not
+    been rounded yet: weights under 1 and a step of lr differ by some half steps of fp32. Later steps go on."""
+    from apex_amd import amp
+    from apex_amd.optimizers import FusedAdam
+
+    first = []
+    for cls in (FusedAdam8bit, FusedAdam):
+        torch.manual_seed(0)
+        net = torch.nn.Sequential(torch.nn.Linear(64, 200), torch.nn.ReLU(), torch.nn.Linear(200, 8)).cuda()
+        opt = cls(net.parameters(), lr=1e-2)
+        net, opt = amp.initialize(net, opt, opt_level=level, cast_model_type=torch.bfloat16, loss_scale=128.0, verbosity=0)
+        x = torch.randn(32, 64, device="cuda")
+        for step in range(3):
+            before = [p.detach().clone() for p in amp.master_params(opt)]
+            loss = net(x).float().square().mean()
+            with amp.scale_loss(loss, opt) as scaled:
+                scaled.backward()
+            opt.step()
+            opt.zero_grad()
+            after = [p.detach().clone() for p in amp.master_params(opt)]
+            assert all(torch.isfinite(p).all() and not torch.equal(p, b) for p, b in zip(after, before))
+            if step == 0:
+                first.append(after)
+    for a, b in zip(*first):
+        # FusedAdam takes 1 - beta2 in fp32, which is 1.3e-5 off, and so is half of it in a step; a weight that is held in
+        # 16 bits may be rounded to the other side
+        assert a.dtype == (torch.float32 if level == "O2" else torch.bfloat16)
+        torch.testing.assert_close(a, b, rtol=torch.finfo(a.dtype).eps + 4 * 2 ** -24, atol=1e-2 * (1.3e-5 + 32 * 2 ** -24))
