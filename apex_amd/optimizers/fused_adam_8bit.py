@@ -261,7 +261,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
         if self.adam_w_mode == 0:
             gf = gf + wd * pf
         mf = beta1 * _decode(flat(m), m_scale) + (1 - beta1) * gf
-        rf = (beta2 * _decode(flat(r), r_scale) ** 2 + (1 - beta2) * gf * gf).sqrt()
+        rf = _decode(flat(r), r_scale)
+        rf = (beta2 * rf * rf + (1 - beta2) * gf * gf).sqrt()  # in the kernel's order
         update = (mf / bc1) / (rf / math.sqrt(bc2) + group["eps"])
         if self.adam_w_mode == 1:
             update = update + wd * pf

@@ -215,6 +215,21 @@ __device__ __forceinline__ float encode_block(const float* x, const unsigned* bi
   return scale;
 }
 
+// The new moments, each product and sum rounded by itself, as elementary operations
+// do it: a code or scale that fell to the other side by a last bit would show in
+// all that follows. (The _rn functions are plain products and sums to the compiler,
+// which fuses them.)
+__device__ __forceinline__ float mean_of(float beta, float m, float rest, float g) {
+#pragma clang fp contract(off)
+  const float old = beta * m, now = rest * g;
+  return old + now;
+}
+__device__ __forceinline__ float square_of(float beta, float r, float rest, float g) {
+#pragma clang fp contract(off)
+  const float old = beta * r * r, now = rest * g * g;
+  return old + now;
+}
+
 template <typename T, bool MASTER>
 __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Adam8Args a) {
   __shared__ float corrections[2];
@@ -298,11 +313,8 @@ __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Ada
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     bits[j] = mix32(((unsigned)i + j) * 0x9E3779B1u + key + high);
-    // each product and sum is rounded by itself, as elementary operations do it: a code or scale that fell to the
-    // other side would show in all that follows
-    m[j] = __fadd_rn(__fmul_rn(a.beta1, __fmul_rn(m[j], sm)), __fmul_rn(a.rest1, g[j]));
-    const float rj = __fmul_rn(r[j], sr);
-    r[j] = root(__fadd_rn(__fmul_rn(__fmul_rn(a.beta2, rj), rj), __fmul_rn(__fmul_rn(a.rest2, g[j]), g[j])));
+    m[j] = mean_of(a.beta1, m[j] * sm, a.rest1, g[j]);
+    r[j] = root(square_of(a.beta2, r[j] * sr, a.rest2, g[j]));
     update[j] = (m[j] * a.bc1_recip) * __builtin_amdgcn_rcpf(fmaf(r[j], a.bc2_root_recip, a.eps));
   }
   if (a.mode == 1) {
