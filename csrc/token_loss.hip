@@ -900,7 +900,7 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
     using std::integral_constant;
     if (packs <= 512) launch(integral_constant<int, 64>{});
     else if (packs <= 1536 && rows >= 1024) launch(integral_constant<int, 128>{});
-    else if (packs < (rows >= 1024 ? 8192 : 3072)) launch(integral_constant<int, 256>{});
+    else if (packs < (rows >= 1024 ? 8192 : 3000)) launch(integral_constant<int, 256>{});
     else launch(integral_constant<int, 512>{});
   }()));
   HIP_CHECK(hipGetLastError());
