@@ -14,6 +14,7 @@ moments before they are rounded. Device path: csrc/multi_tensor_adam_8bit.hip. C
 import math
 
 import torch
+from torch.amp.grad_scaler import OptState
 
 from .._ext import get_ext
 from ..tracing import traced
@@ -219,8 +220,12 @@ class FusedAdam8bit(torch.optim.Optimizer):
         if grad_scaler is None:
             group["step"].add_(1)  # in place: a hipGraph's replay has to see it
             return None, None
-        found_inf = grad_scaler._check_inf_per_device(self)[device].float()
-        inv_scale = grad_scaler._get_scale_async().double().reciprocal().float()
+        state = grad_scaler._per_optimizer_states[id(self)]
+        if state["stage"] is OptState.UNSCALED:  # unscale_ has divided the gradients, and kept what it found
+            found_inf, inv_scale = state["found_inf_per_device"][device].float(), None
+        else:
+            found_inf = grad_scaler._check_inf_per_device(self)[device].float()
+            inv_scale = grad_scaler._get_scale_async().double().reciprocal().float()
         group["step"].add_((found_inf == 0).to(torch.int32))
         return found_inf, inv_scale
 

@@ -208,3 +208,38 @@ def test_refusals():
     s.grad = torch.zeros(4, 3)
     with pytest.raises(RuntimeError, match="dense"):
         FusedAdam8bit([s]).step()
+
+
+@pytest.mark.parametrize("unscale", [False, True])
+def test_a_scaler_that_has_unscaled_already(unscale):
+    """unscale_, clip, step: the step is that of the true gradients, bit for bit (the scale is a power of two), at an eps
+    that tells their size; one that is not finite skips it and does not count."""
+    g = torch.Generator().manual_seed(4)
+    start = [torch.randn(s, generator=g) for s in ((3, 50), (129,))]
+    args = dict(lr=1e-2, eps=1e-2, capturable=True, master_weights=True)
+    pa, pb = ([torch.nn.Parameter(w.clone()) for w in start] for _ in range(2))
+    a, b = (FusedAdam8bit([{"params": p[:1]}, {"params": p[1:]}], **args) for p in (pa, pb))
+    scaler = torch.amp.GradScaler("cpu", init_scale=1024.0, growth_interval=1000)
+    scaler.scale(torch.zeros(()))
+    for step in range(3):
+        for p, q in zip(pa, pb):
+            d = 0.02 * torch.randn(p.shape, generator=g)
+            p.grad, q.grad = d * 1024, d
+        if step == 1:
+            pa[1].grad[7] = math.inf
+        if unscale:
+            scaler.unscale_(a)
+            for x in (pa, pb):
+                torch.nn.utils.clip_grad_norm_(x, 0.1)
+        before = [p.detach().clone() for p in pa]
+        scaler.step(a)
+        scaler.update(1024.0)
+        if step == 1:
+            assert all(torch.equal(p, w) for p, w in zip(pa, before))
+        else:
+            b.step()
+        assert [int(x["step"]) for x in a.param_groups] == [(1, 1, 2)[step]] * 2
+        for p, q in zip(pa, pb):
+            assert torch.equal(p, q)
+            for k in a.state[p]:
+                assert torch.equal(a.state[p][k].view(torch.uint8), b.state[q][k].view(torch.uint8))

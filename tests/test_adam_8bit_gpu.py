@@ -423,3 +423,37 @@ def test_under_amp(level):
         # 16 bits may be rounded to the other side
         assert a.dtype == (torch.float32 if level == "O2" else torch.bfloat16)
         torch.testing.assert_close(a, b, rtol=torch.finfo(a.dtype).eps + 4 * 2 ** -24, atol=1e-2 * (1.3e-5 + 32 * 2 ** -24))
+
+
+@pytest.mark.parametrize("unscale", [False, True])
+def test_a_scaler_that_has_unscaled_already(unscale):
+    """unscale_, clip, step: the step is that of the true gradients, bit for bit (the scale is a power of two), at an eps
+    that tells their size; one that is not finite skips it and does not count."""
+    sizes = [(3, 50), (129,), (5000,)]
+    pa, _ = make(sizes, torch.float32, device="cuda")
+    pb, gb = make(sizes, torch.float32, device="cuda")
+    a, b = (FusedAdam8bit([{"params": p[:1]}, {"params": p[1:]}], lr=1e-2, eps=1e-2, capturable=True) for p in (pa, pb))
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0, growth_interval=1000)
+    scaler.scale(torch.zeros((), device="cuda"))
+    for step in range(3):
+        gb(step)
+        for p, q in zip(pa, pb):
+            p.grad = q.grad * 1024
+        if step == 1:
+            pa[1].grad[7] = math.inf
+        if unscale:
+            scaler.unscale_(a)
+            for x in (pa, pb):
+                torch.nn.utils.clip_grad_norm_(x, 0.1)
+        before = [p.detach().clone() for p in pa]
+        scaler.step(a)
+        scaler.update(1024.0)
+        if step == 1:
+            assert all(torch.equal(p, w) for p, w in zip(pa, before))
+        else:
+            b.step()
+        assert [int(x["step"]) for x in a.param_groups] == [(1, 1, 2)[step]] * 2
+        for p, q in zip(pa, pb):
+            assert torch.equal(p, q)
+            for k in a.state[p]:
+                assert torch.equal(a.state[p][k].view(torch.uint8), b.state[q][k].view(torch.uint8))
