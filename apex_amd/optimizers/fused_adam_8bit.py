@@ -172,6 +172,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
 
+        founds, unscale = self._asked(grad_scaler)
         first = 0  # a tensor's place in the optimizer is part of its random numbers
         for group in self.param_groups:
             params = group["params"]
@@ -194,7 +195,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
                 else:
                     lists[key] = [row]
             first += len(params)
-            found_inf, inv_scale = self._count(group, grad_scaler)
+            found_inf, inv_scale = self._count(group, founds, unscale)
             for (device, _, master), rows in lists.items():
                 names = _STATE + (("master_param",) if master else ())
                 if device.type == "cuda":
@@ -207,8 +208,17 @@ class FusedAdam8bit(torch.optim.Optimizer):
                         self._step_ref(group, place, inv_scale, grad, p, *(state[name] for name in names))
         return loss
 
-    def _count(self, group, grad_scaler):
-        """Advances the group's step; what GradScaler has for it, on the device."""
+    def _asked(self, grad_scaler):
+        """What GradScaler found on each device (it looks at all gradients: once a step), and 1 / scale."""
+        if grad_scaler is None or not self.capturable:
+            return None, None
+        state = grad_scaler._per_optimizer_states[id(self)]
+        if state["stage"] is OptState.UNSCALED:  # unscale_ has divided the gradients, and kept what it found
+            return state["found_inf_per_device"], None
+        return grad_scaler._check_inf_per_device(self), grad_scaler._get_scale_async().double().reciprocal().float()
+
+    def _count(self, group, founds, inv_scale):
+        """Advances the group's step; what GradScaler has for it, on its device."""
         if not self.capturable:
             group["step"] = group.get("step", 0) + 1
             return None, None
@@ -217,17 +227,12 @@ class FusedAdam8bit(torch.optim.Optimizer):
             group["step"] = torch.zeros(1, dtype=torch.int32, device=device)
         if torch.is_tensor(group["lr"]) and group["lr"].device != device:
             group["lr"] = group["lr"].to(device)
-        if grad_scaler is None:
+        if not founds:
             group["step"].add_(1)  # in place: a hipGraph's replay has to see it
             return None, None
-        state = grad_scaler._per_optimizer_states[id(self)]
-        if state["stage"] is OptState.UNSCALED:  # unscale_ has divided the gradients, and kept what it found
-            found_inf, inv_scale = state["found_inf_per_device"][device].float(), None
-        else:
-            found_inf = grad_scaler._check_inf_per_device(self)[device].float()
-            inv_scale = grad_scaler._get_scale_async().double().reciprocal().float()
+        found_inf = founds[device].float()
         group["step"].add_((found_inf == 0).to(torch.int32))
-        return found_inf, inv_scale
+        return found_inf, inv_scale if inv_scale is None else inv_scale.to(device)
 
     # ----- device path -----
     def _step_cuda(self, group, places, tensors, found_inf, inv_scale):

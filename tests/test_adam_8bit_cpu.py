@@ -243,3 +243,22 @@ def test_a_scaler_that_has_unscaled_already(unscale):
             assert torch.equal(p, q)
             for k in a.state[p]:
                 assert torch.equal(a.state[p][k].view(torch.uint8), b.state[q][k].view(torch.uint8))
+
+
+def test_a_scaler_is_asked_once_for_a_step():
+    """Whatever the number of groups: each question reads and writes all gradients. After unscale_ it is not asked."""
+    params = [torch.nn.Parameter(torch.ones(5)) for _ in range(3)]
+    opt = FusedAdam8bit([{"params": [p]} for p in params], capturable=True)
+    scaler, asked = torch.amp.GradScaler("cpu", init_scale=4.0), []
+    scaler.scale(torch.zeros(()))
+    check = scaler._check_inf_per_device
+    scaler._check_inf_per_device = lambda o: (asked.append(o), check(o))[1]
+    for unscale, times in ((False, 1), (True, 1)):
+        for p in params:
+            p.grad = torch.ones(5)
+        if unscale:
+            scaler.unscale_(opt)
+        scaler.step(opt)
+        scaler.update()
+        assert len(asked) == times
+    assert [int(g["step"]) for g in opt.param_groups] == [2, 2, 2]
