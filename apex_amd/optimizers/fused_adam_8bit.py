@@ -214,8 +214,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
             return None, None
         state = grad_scaler._per_optimizer_states[id(self)]
         if state["stage"] is OptState.UNSCALED:  # unscale_ has divided the gradients, and kept what it found
-            return state["found_inf_per_device"], None
-        return grad_scaler._check_inf_per_device(self), grad_scaler._get_scale_async().double().reciprocal().float()
+            return list(state["found_inf_per_device"].values()), None
+        return list(grad_scaler._check_inf_per_device(self).values()), grad_scaler._get_scale_async().double().reciprocal().float()
 
     def _count(self, group, founds, inv_scale):
         """Advances the group's step; what GradScaler has for it, on its device."""
@@ -230,7 +230,9 @@ class FusedAdam8bit(torch.optim.Optimizer):
         if not founds:
             group["step"].add_(1)  # in place: a hipGraph's replay has to see it
             return None, None
-        found_inf = founds[device].float()
+        # a gradient on any device that is not finite skips the step on all
+        found = [f.to(device=device, dtype=torch.float32) for f in founds]
+        found_inf = found[0] if len(found) == 1 else torch.stack(found).amax(0)
         group["step"].add_((found_inf == 0).to(torch.int32))
         return found_inf, inv_scale if inv_scale is None else inv_scale.to(device)
 

@@ -262,3 +262,22 @@ def test_a_scaler_is_asked_once_for_a_step():
         scaler.update()
         assert len(asked) == times
     assert [int(g["step"]) for g in opt.param_groups] == [2, 2, 2]
+
+
+def test_what_one_device_found_holds_for_all():
+    """Params on several devices: one gradient that is not finite skips the step of each (the scaler's record of another
+    device is made up here)."""
+    from torch.amp.grad_scaler import OptState
+
+    p = torch.nn.Parameter(torch.ones(5))
+    opt = FusedAdam8bit([p], capturable=True)
+    scaler = torch.amp.GradScaler("cpu")
+    scaler.scale(torch.zeros(()))
+    for found in (1.0, 0.0):
+        p.grad = torch.ones(5)
+        scaler._per_optimizer_states[id(opt)] = {
+            "stage": OptState.UNSCALED,
+            "found_inf_per_device": {torch.device("cpu"): torch.tensor(0.0), torch.device("cpu", 1): torch.tensor(found)},
+        }
+        opt.step(grad_scaler=scaler)
+        assert torch.equal(p.detach(), torch.ones(5)) == bool(found) and int(opt.param_groups[0]["step"]) == 1 - int(found)

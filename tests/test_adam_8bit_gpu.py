@@ -457,3 +457,22 @@ def test_a_scaler_that_has_unscaled_already(unscale):
             assert torch.equal(p, q)
             for k in a.state[p]:
                 assert torch.equal(a.state[p][k].view(torch.uint8), b.state[q][k].view(torch.uint8))
+
+
+def test_what_one_device_found_holds_for_all():
+    """Params on the GPU and on the CPU: a gradient on either that is not finite skips both."""
+    p, q = (torch.nn.Parameter(torch.ones(200, device=d)) for d in ("cuda", "cpu"))
+    opt = FusedAdam8bit([{"params": [p]}, {"params": [q]}], lr=1e-2, capturable=True)
+    scaler = torch.amp.GradScaler("cuda", init_scale=64.0, growth_interval=1000)
+    scaler.scale(torch.zeros((), device="cuda"))
+    for bad in (p, q, None):
+        for w in (p, q):
+            w.grad = torch.full_like(w, 64.0 * 0.25)
+        if bad is not None:
+            bad.grad[3] = math.inf
+        scaler.step(opt)
+        scaler.update(64.0)
+        for w in (p, q):
+            assert torch.equal(w.detach(), torch.ones_like(w)) == (bad is not None)
+    assert [int(g["step"]) for g in opt.param_groups] == [1, 1]
+    torch.testing.assert_close(p.detach().cpu(), q.detach(), rtol=0, atol=4 * 2 ** -24)
