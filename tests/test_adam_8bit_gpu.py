@@ -476,3 +476,29 @@ def test_what_one_device_found_holds_for_all():
             assert torch.equal(w.detach(), torch.ones_like(w)) == (bad is not None)
     assert [int(g["step"]) for g in opt.param_groups] == [1, 1]
     torch.testing.assert_close(p.detach().cpu(), q.detach(), rtol=0, atol=4 * 2 ** -24)
+
+
+@pytest.mark.parametrize("size", [2e-21, 1e-20, 1e-19, 1e-18, 3e-18, 1e-17, 1e-14, 1e19, 5.8e20, 7e20, 1e30, 3e38])
+def test_the_root_at_both_ends(size):
+    """Second moments that are subnormal or just over it (gradients up to some 1e-17), close to fp32's largest (5.8e20)
+    and infinite (from 5.83e20 on: their code is NaN, and the step is m / inf = 0), beside gradients of 0. v and m are the
+    same operations on both sides; the root, the quotient and the products are off by under 16 half steps together."""
+    g = size * (1 + torch.rand(300, generator=torch.Generator().manual_seed(0)) / 64)
+    g[::7] = 0
+    g.clamp_(max=torch.finfo(torch.float32).max)
+    out = []
+    for device in ("cuda", "cpu"):
+        p = torch.nn.Parameter(torch.zeros(300, device=device))
+        opt = FusedAdam8bit([p], lr=1e-2, eps=1e-30, bias_correction=False)
+        p.grad = g.to(device)
+        opt.step()
+        out.append((p.detach().cpu(), {k: v.cpu() for k, v in opt.state[p].items()}))
+    (p, s), (q, t) = out
+    torch.testing.assert_close(p, q, rtol=16 * 2 ** -24, atol=0)
+    over = (torch.tensor(1 - 0.999, dtype=torch.float32) * g * g).isinf()
+    assert torch.equal(t["exp_avg_sq"].float().isnan(), over) and torch.equal(p == 0, over | (g == 0))
+    for k in ("exp_avg", "exp_avg_sq"):
+        torch.testing.assert_close(s[k + "_scale"], t[k + "_scale"], rtol=8 * 2 ** -24, atol=0)
+        # a code by one where a value lies within those half steps of its threshold: hardly ever
+        a, b = s[k].float(), t[k].float()
+        assert torch.equal(a.isnan(), b.isnan()) and (a.nan_to_num() != b.nan_to_num()).sum() <= 2
