@@ -73,6 +73,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
 
     Arguments are those of :class:`FusedAdam`, and
 
+    - lr: with ``capturable`` a number becomes a tensor of each param group, to be changed in place; a tensor is used as
+      it is, by all groups that set no other.
     - master_weights (bool): keep fp32 copies of fp16/bf16 params and step those (with or without ``capturable``).
       A step far smaller than a param's own spacing is lost without them.
     - seed (int): of the random rounding. Ranks that hold the same params need the same seed.
@@ -106,19 +108,24 @@ class FusedAdam8bit(torch.optim.Optimizer):
             raise ValueError(f"betas must be in [0, 1), got {betas}")
         if not eps >= 0.0:
             raise ValueError(f"eps must not be negative, got {eps}")
-        if capturable and not torch.is_tensor(lr):
-            # the kernel reads it on the device, so that a hipGraph's replay sees new values
-            lr = torch.tensor(lr, dtype=torch.float32)
-            if torch.cuda.is_available():
-                lr = lr.cuda()
+        self.capturable = capturable  # groups are added by it
         defaults = dict(lr=lr, bias_correction=bias_correction, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
         self.adam_w_mode = 1 if adam_w_mode else 0
         self.set_grad_none = set_grad_none
-        self.capturable = capturable
         self.master_weights = master_weights
         self.seed = int(seed)
         self._step_supports_amp_scaling = capturable
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        if self.capturable and not torch.is_tensor(group["lr"]):
+            # the kernel reads it on the device, so that a hipGraph's replay sees new values; schedules write it in
+            # place, so each group has its own
+            params = group["params"]
+            device = params[0].device if params else "cuda" if torch.cuda.is_available() else "cpu"
+            group["lr"] = torch.tensor(group["lr"], dtype=torch.float32, device=device)
 
     def zero_grad(self, set_to_none: bool = True):
         super().zero_grad(set_to_none=self.set_grad_none or set_to_none)
@@ -145,7 +152,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
                     for key, dtype in (("lr", torch.float32), ("step", torch.int32)):
                         v = group.get(key)
                         if v is not None:
-                            group[key] = torch.as_tensor(v, dtype=dtype, device=device)
+                            group[key] = torch.as_tensor(v, dtype=dtype, device=device).clone()  # groups may share it
         else:
             for group in self.param_groups:
                 for key in ("lr", "step"):

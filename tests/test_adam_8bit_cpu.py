@@ -281,3 +281,49 @@ def test_what_one_device_found_holds_for_all():
         }
         opt.step(grad_scaler=scaler)
         assert torch.equal(p.detach(), torch.ones(5)) == bool(found) and int(opt.param_groups[0]["step"]) == 1 - int(found)
+
+
+def test_each_group_has_a_learning_rate_of_its_own():
+    """A schedule writes tensor rates in place: one that two groups share would hold the last group's value."""
+    params = [torch.nn.Parameter(torch.zeros(5)) for _ in range(4)]
+    opt = FusedAdam8bit([{"params": params[:1]}, {"params": params[1:2]}, {"params": params[2:3], "lr": 0.5}], lr=1e-2, capturable=True)
+    opt.add_param_group({"params": params[3:]})
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, [lambda e, f=f: f for f in (1.0, 0.1, 0.01, 0.001)])
+    want = [1e-2, 1e-3, 5e-3, 1e-5]
+
+    def rates(o):
+        assert all(torch.is_tensor(g["lr"]) and g["lr"].dtype == torch.float32 for g in o.param_groups)
+        return [g["lr"].item() for g in o.param_groups]
+
+    assert rates(opt) == pytest.approx(want)
+    for p in params:
+        p.grad = torch.ones(5)
+    opt.step()
+    # m / root(v) is 1 in the first step
+    assert [-p[0].item() for p in params] == pytest.approx(want, rel=1e-5)
+    schedule.step()
+    assert rates(opt) == pytest.approx(want)
+    other = FusedAdam8bit([{"params": [torch.nn.Parameter(torch.zeros(5))]} for _ in range(4)], lr=1.0, capturable=True)
+    other.load_state_dict(opt.state_dict())
+    assert rates(other) == pytest.approx(want)
+    other.param_groups[0]["lr"].fill_(7.0)
+    assert rates(other) == pytest.approx([7.0] + want[1:])
+    # a checkpoint of groups that share one tensor
+    saved = opt.state_dict()
+    for g in saved["param_groups"]:
+        g["lr"] = opt.param_groups[0]["lr"]
+    other.load_state_dict(saved)
+    other.param_groups[0]["lr"].fill_(7.0)
+    assert rates(other) == pytest.approx([7.0, 1e-2, 1e-2, 1e-2])
+
+
+def test_a_learning_rate_that_the_caller_holds():
+    """A tensor that the caller gives is used as it is, by every group without a rate of its own: what torch does."""
+    params = [torch.nn.Parameter(torch.zeros(5)) for _ in range(2)]
+    lr = torch.tensor(1e-2)
+    opt = FusedAdam8bit([{"params": [p]} for p in params], lr=lr, capturable=True)
+    lr.fill_(3e-3)
+    for p in params:
+        p.grad = torch.ones(5)
+    opt.step()
+    assert [-p[0].item() for p in params] == pytest.approx([3e-3, 3e-3], rel=1e-5)
