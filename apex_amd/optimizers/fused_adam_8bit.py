@@ -81,7 +81,9 @@ class FusedAdam8bit(torch.optim.Optimizer):
 
     Per param, ``state`` holds ``exp_avg`` and ``exp_avg_sq`` (``float8_e4m3fn`` codes of the param's shape;
     ``exp_avg_sq`` the root of the second moment), ``exp_avg_scale`` and ``exp_avg_sq_scale`` (fp32, one for each 128
-    elements in memory order) and with ``master_weights`` ``master_param``. ``state_dict`` keeps them as they are.
+    elements in memory order) and with ``master_weights`` ``master_param``. ``state_dict`` keeps them as they are. After a
+    checkpoint without masters, ``master_weights`` makes them from the params in the first step; without it, a
+    checkpoint's are left out.
 
     Unlike :class:`FusedAdam` with ``capturable``, gradients are left as they are (not overwritten unscaled), and a
     step that GradScaler skips does not count.
@@ -144,6 +146,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
                 self.state[p] = {
                     name: v.to(device=p.device).clone(memory_format=torch.preserve_format) if torch.is_tensor(v) else v
                     for name, v in saved[k].items()
+                    if name != "master_param" or self.master_weights
                 }
         if self.capturable:
             for group in self.param_groups:
@@ -168,8 +171,12 @@ class FusedAdam8bit(torch.optim.Optimizer):
         for name in ("exp_avg", "exp_avg_sq"):
             state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
             state[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-        if self.master_weights and p.dtype != torch.float32:
-            state["master_param"] = p.detach().float().clone()
+
+    def _init_master(self, p, state):
+        # captured, the copy would be made anew at every replay
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdam8bit makes master weights in its first step (after loading, too): take one before capture")
+        state["master_param"] = p.detach().float().clone()
 
     @torch.no_grad()
     @traced("FusedAdam8bit.step")
@@ -195,6 +202,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     self._init_state(p, state)
+                if self.master_weights and "master_param" not in state and p.dtype != torch.float32:
+                    self._init_master(p, state)  # new, or loaded from a checkpoint without
                 key = p.device, p.dtype, "master_param" in state
                 row = place, grad, p, state
                 if key in lists:

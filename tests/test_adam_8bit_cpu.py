@@ -327,3 +327,37 @@ def test_a_learning_rate_that_the_caller_holds():
         p.grad = torch.ones(5)
     opt.step()
     assert [-p[0].item() for p in params] == pytest.approx([3e-3, 3e-3], rel=1e-5)
+
+
+def test_a_checkpoint_without_masters_gets_them_and_one_with_them_loses_them():
+    """master_weights is the loading optimizer's to say. 2 - 1e-5 is no bf16: without masters the weight never moves."""
+    def go(opt, p, steps):
+        for _ in range(steps):
+            p.grad = torch.ones_like(p)
+            opt.step()
+
+    def new(master):
+        p = torch.nn.Parameter(torch.ones(200, dtype=torch.bfloat16))
+        return p, FusedAdam8bit([p], lr=1e-5, master_weights=master)
+
+    p, without = new(False)
+    go(without, p, 2)
+    q, opt = new(True)
+    opt.load_state_dict(without.state_dict())
+    with torch.no_grad():
+        q.fill_(2.0)  # the weights may be loaded after the optimizer
+    go(opt, q, 5)
+    # the same from a checkpoint that has them
+    saved = without.state_dict()
+    saved["state"][0] = saved["state"][0] | {"master_param": torch.full((200,), 2.0)}
+    w, other = new(True)
+    other.load_state_dict(saved)
+    go(other, w, 5)
+    master = opt.state[q]["master_param"]
+    assert master.dtype == torch.float32 and (master < 2.0 - 3e-5).all()
+    assert torch.equal(master, other.state[w]["master_param"]) and torch.equal(q.detach(), master.bfloat16())
+    r, back = new(False)
+    back.load_state_dict(opt.state_dict())
+    go(back, r, 2)
+    assert "master_param" not in back.state[r] and torch.equal(r.detach(), torch.ones(200, dtype=torch.bfloat16))
+    assert "master_param" in opt.state[q]

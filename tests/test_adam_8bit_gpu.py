@@ -502,3 +502,30 @@ def test_the_root_at_both_ends(size):
         # a code by one where a value lies within those half steps of its threshold: hardly ever
         a, b = s[k].float(), t[k].float()
         assert torch.equal(a.isnan(), b.isnan()) and (a.nan_to_num() != b.nan_to_num()).sum() <= 2
+
+
+def test_masters_after_a_checkpoint_without_them():
+    """Made in the first eager step, and the step is the CPU path's; a capture that would make them is refused."""
+    pa, ga = make([(300,), (77, 5)], torch.bfloat16, device="cuda")
+    a = FusedAdam8bit(pa, lr=1e-2, capturable=True)
+    ga(0)
+    a.step()
+    for capture in (True, False):
+        pb, gb = make([(300,), (77, 5)], torch.bfloat16, device="cuda")
+        b = FusedAdam8bit(pb, lr=1e-2, capturable=True, master_weights=True)
+        b.load_state_dict(a.state_dict())
+        gb(1)
+        if not capture:
+            b.step()
+            continue
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="before capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                b.step()
+    pc, gc = make([(300,), (77, 5)], torch.bfloat16)
+    c = FusedAdam8bit(pc, lr=1e-2, master_weights=True)
+    c.load_state_dict(a.state_dict())
+    gc(1)
+    c.step()
+    same(b, c, pb, pc, 1e-2, torch.bfloat16)
+    assert all(torch.equal(p.detach(), b.state[p]["master_param"].bfloat16()) for p in pb)
