@@ -68,6 +68,12 @@ def _encode(x, u, root):
     return q.to(torch.float8_e4m3fn), scales
 
 
+def _check_not_captured(device):
+    """Before state is made: captured, it would be made anew at every replay."""
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("FusedAdam8bit makes its state, and after loading its masters, in a first step: take one before capture")
+
+
 class FusedAdam8bit(torch.optim.Optimizer):
     """Adam/AdamW with 8-bit moments in a single fused multi-tensor HIP kernel.
 
@@ -167,15 +173,14 @@ class FusedAdam8bit(torch.optim.Optimizer):
             raise RuntimeError("FusedAdam8bit only supports fp16/bf16/fp32 params")
         if torch.empty_like(p, device="meta").stride() != p.stride():
             raise RuntimeError("FusedAdam8bit only supports dense params without gaps or overlaps")
+        _check_not_captured(p.device)
         blocks = -(-p.numel() // BLOCK)
         for name in ("exp_avg", "exp_avg_sq"):
             state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
             state[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
 
     def _init_master(self, p, state):
-        # captured, the copy would be made anew at every replay
-        if p.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("FusedAdam8bit makes master weights in its first step (after loading, too): take one before capture")
+        _check_not_captured(p.device)
         state["master_param"] = p.detach().float().clone()
 
     @torch.no_grad()
@@ -240,6 +245,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
             return None, None
         device = group["params"][0].device
         if "step" not in group:
+            _check_not_captured(device)
             group["step"] = torch.zeros(1, dtype=torch.int32, device=device)
         if torch.is_tensor(group["lr"]) and group["lr"].device != device:
             group["lr"] = group["lr"].to(device)

@@ -529,3 +529,25 @@ def test_masters_after_a_checkpoint_without_them():
     c.step()
     same(b, c, pb, pc, 1e-2, torch.bfloat16)
     assert all(torch.equal(p.detach(), b.state[p]["master_param"].bfloat16()) for p in pb)
+
+
+def test_a_first_step_is_not_captured():
+    """Its state would be made anew, with moments of 0 and step 1, at every replay: refused, also where only one param
+    meets its first gradient, and what was there stays."""
+    pa, ga = make([(300,), (77, 5)], torch.float32, device="cuda")
+    opt = FusedAdam8bit(pa, lr=1e-2, capturable=True)
+    for taken in (False, True):
+        ga(0)
+        if taken:
+            pa[1].grad = None
+            opt.step()
+            ga(1)
+        before = [p.detach().clone() for p in pa]
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="before capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                opt.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, b) for p, b in zip(pa, before))
+    opt.step()
+    assert len(opt.state) == 2 and int(opt.param_groups[0]["step"]) == 2
