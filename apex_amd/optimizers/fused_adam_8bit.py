@@ -240,10 +240,12 @@ class FusedAdam8bit(torch.optim.Optimizer):
 
     def _count(self, group, founds, inv_scale):
         """Advances the group's step; what GradScaler has for it, on its device."""
+        device = group["params"][0].device
         if not self.capturable:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdam8bit needs capturable=True to be captured: replays would repeat one step's numbers")
             group["step"] = group.get("step", 0) + 1
             return None, None
-        device = group["params"][0].device
         if "step" not in group:
             _check_not_captured(device)
             group["step"] = torch.zeros(1, dtype=torch.int32, device=device)

@@ -551,3 +551,17 @@ def test_a_first_step_is_not_captured():
         assert all(torch.equal(p, b) for p, b in zip(pa, before))
     opt.step()
     assert len(opt.state) == 2 and int(opt.param_groups[0]["step"]) == 2
+
+
+def test_a_capture_needs_capturable():
+    """Without it step, lr and the random numbers of the rounding would be the captured step's for ever."""
+    pa, ga = make([(300,)], torch.float32, device="cuda")
+    opt = FusedAdam8bit(pa, lr=1e-2)
+    ga(0)
+    opt.step()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert opt.param_groups[0]["step"] == 1
+    opt.step()
