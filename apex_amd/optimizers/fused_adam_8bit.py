@@ -83,7 +83,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
       it is, by all groups that set no other.
     - master_weights (bool): keep fp32 copies of fp16/bf16 params and step those (with or without ``capturable``).
       A step far smaller than a param's own spacing is lost without them.
-    - seed (int): of the random rounding. Ranks that hold the same params need the same seed.
+    - seed (int): of the random rounding, kept in the param groups and so in checkpoints. Ranks that hold the same params
+      need the same seed.
 
     Per param, ``state`` holds ``exp_avg`` and ``exp_avg_sq`` (``float8_e4m3fn`` codes of the param's shape;
     ``exp_avg_sq`` the root of the second moment), ``exp_avg_scale`` and ``exp_avg_sq_scale`` (fp32, one for each 128
@@ -117,12 +118,12 @@ class FusedAdam8bit(torch.optim.Optimizer):
         if not eps >= 0.0:
             raise ValueError(f"eps must not be negative, got {eps}")
         self.capturable = capturable  # groups are added by it
-        defaults = dict(lr=lr, bias_correction=bias_correction, betas=betas, eps=eps, weight_decay=weight_decay)
+        defaults = dict(lr=lr, bias_correction=bias_correction, betas=betas, eps=eps, weight_decay=weight_decay,
+                        seed=int(seed))
         super().__init__(params, defaults)
         self.adam_w_mode = 1 if adam_w_mode else 0
         self.set_grad_none = set_grad_none
         self.master_weights = master_weights
-        self.seed = int(seed)
         self._step_supports_amp_scaling = capturable
 
     def add_param_group(self, param_group):
@@ -154,6 +155,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
                     for name, v in saved[k].items()
                     if name != "master_param" or self.master_weights
                 }
+        for group in self.param_groups:
+            group.setdefault("seed", self.defaults["seed"])  # of a checkpoint that does not keep it
         if self.capturable:
             for group in self.param_groups:
                 if group["params"]:
@@ -271,11 +274,11 @@ class FusedAdam8bit(torch.optim.Optimizer):
                 lr = group["lr"] = torch.tensor(lr, dtype=torch.float32, device=tensors[0][0].device)
             amp_C.multi_tensor_adam_8bit_capturable(
                 tensors, places, lr.float(), beta1, beta2, group["eps"], group["step"], self.adam_w_mode,
-                bias_correction, group["weight_decay"], self.seed & _MASK, inv_scale, found_inf)
+                bias_correction, group["weight_decay"], group["seed"] & _MASK, inv_scale, found_inf)
         else:
             amp_C.multi_tensor_adam_8bit(
                 tensors, places, float(group["lr"]), beta1, beta2, group["eps"], group["step"], self.adam_w_mode,
-                bias_correction, group["weight_decay"], self.seed & _MASK)
+                bias_correction, group["weight_decay"], group["seed"] & _MASK)
 
     # ----- reference path (CPU CI + numerics oracle) -----
     def _step_ref(self, group, place, inv_scale, g, p, m, m_scale, r, r_scale, master=None):
@@ -291,7 +294,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
         n = p.numel()
         if n == 0:
             return
-        bits = _random_bits(self.seed, step, place, n)
+        bits = _random_bits(group["seed"], step, place, n)
         gf = flat(g).float() * (1.0 if inv_scale is None else float(inv_scale))
         pf = flat(p if master is None else master).float()
         if self.adam_w_mode == 0:

@@ -361,3 +361,36 @@ def test_a_checkpoint_without_masters_gets_them_and_one_with_them_loses_them():
     go(back, r, 2)
     assert "master_param" not in back.state[r] and torch.equal(r.detach(), torch.ones(200, dtype=torch.bfloat16))
     assert "master_param" in opt.state[q]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_checkpoint_brings_its_seed(capturable):
+    """The random numbers go on as they would have, whatever seed the loading optimizer was made with; a checkpoint
+    from before seeds were kept leaves it its own."""
+    g = torch.Generator().manual_seed(5)
+    grads = [torch.randn(300, generator=g) for _ in range(4)]
+
+    def go(opt, p, gs):
+        for x in gs:
+            p.grad = x.clone()
+            opt.step()
+
+    def new(seed):
+        p = torch.nn.Parameter(torch.zeros(300))
+        return p, FusedAdam8bit([p], lr=1e-2, seed=seed, capturable=capturable)
+
+    p, opt = new(9)
+    go(opt, p, grads[:2])
+    saved, start = copy.deepcopy(opt.state_dict()), p.detach().clone()
+    go(opt, p, grads[2:])
+    old = copy.deepcopy(saved)
+    assert old["param_groups"][0].pop("seed") == 9
+    for state, seed in ((saved, 0), (old, 9)):
+        q, other = new(seed)
+        with torch.no_grad():
+            q.copy_(start)
+        other.load_state_dict(state)
+        go(other, q, grads[2:])
+        assert torch.equal(p.detach(), q.detach())
+        for k in opt.state[p]:
+            assert torch.equal(opt.state[p][k].view(torch.uint8), other.state[q][k].view(torch.uint8))
