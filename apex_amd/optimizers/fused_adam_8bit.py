@@ -74,6 +74,30 @@ def _check_not_captured(device):
         raise RuntimeError("FusedAdam8bit makes its state, and after loading its masters, in a first step: take one before capture")
 
 
+def _check_loaded(state, p):
+    """Codes are met in memory order with a scale for each block: they have to lie as the param does."""
+    if not all(k in state for k in _STATE):
+        raise ValueError(f"FusedAdam8bit needs the state {_STATE} for each param, got {tuple(state)}")
+    for name in _STATE + ("master_param",) * ("master_param" in state):
+        v = state[name]
+        scales = name.endswith("_scale")
+        if v.dtype != (torch.float8_e4m3fn if name in ("exp_avg", "exp_avg_sq") else torch.float32):
+            raise ValueError(f"FusedAdam8bit: {name} of a checkpoint is {v.dtype}")
+        if v.shape != ((-(-p.numel() // BLOCK),) if scales else p.shape):
+            raise ValueError(f"FusedAdam8bit: {name} of a checkpoint has shape {tuple(v.shape)} where the param's shape and "
+                             f"layout are {tuple(p.shape)} and {p.stride()}")
+        if not scales and any(n > 1 and a != b for n, a, b in zip(p.shape, v.stride(), p.stride())):
+            raise ValueError(f"FusedAdam8bit: {name} of a checkpoint has another layout than the param: strides {v.stride()}, "
+                             f"not {p.stride()}")
+
+
+def _like(v, p):
+    """A copy of state on the param's device; what has its shape gets its strides."""
+    if v.shape != p.shape:
+        return v.to(device=p.device).clone(memory_format=torch.preserve_format)
+    return torch.empty_like(p, dtype=v.dtype, requires_grad=False).copy_(v)
+
+
 class FusedAdam8bit(torch.optim.Optimizer):
     """Adam/AdamW with 8-bit moments in a single fused multi-tensor HIP kernel.
 
@@ -142,16 +166,16 @@ class FusedAdam8bit(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         # torch casts state to the params' type: the codes and scales are put back as they were saved
         saved = state_dict["state"]
-        for state in saved.values():
-            if state and not all(k in state for k in _STATE):
-                raise ValueError(f"FusedAdam8bit needs the state {_STATE} for each param, got {tuple(state)}")
-        super().load_state_dict(state_dict)
         order = [k for g in state_dict["param_groups"] for k in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for k, p in zip(order, params):
+            if saved.get(k):
+                _check_loaded(saved[k], p)
+        super().load_state_dict(state_dict)
+        for k, p in zip(order, params):
             if k in saved:
                 self.state[p] = {
-                    name: v.to(device=p.device).clone(memory_format=torch.preserve_format) if torch.is_tensor(v) else v
+                    name: _like(v, p) if torch.is_tensor(v) else v
                     for name, v in saved[k].items()
                     if name != "master_param" or self.master_weights
                 }

@@ -394,3 +394,37 @@ def test_a_checkpoint_brings_its_seed(capturable):
         assert torch.equal(p.detach(), q.detach())
         for k in opt.state[p]:
             assert torch.equal(opt.state[p][k].view(torch.uint8), other.state[q][k].view(torch.uint8))
+
+
+def test_a_checkpoint_of_other_params_is_refused():
+    """Codes are met in memory order with a scale for each 128: those of another shape or layout, or without all their
+    scales, would be taken for other elements'. Dimensions of one element have no layout."""
+    w = torch.randn(8, 3, 5, 5, generator=torch.Generator().manual_seed(6))
+
+    def saved(p):
+        opt = FusedAdam8bit([p])
+        p.grad = torch.ones_like(p)
+        opt.step()
+        return opt.state_dict()
+
+    last = torch.nn.Parameter(w.to(memory_format=torch.channels_last))
+    for p, q in ((last, w), (torch.nn.Parameter(w.clone()), w.to(memory_format=torch.channels_last)),
+                 (torch.nn.Parameter(w.reshape(3, 8, 5, 5)), w)):
+        opt = FusedAdam8bit([torch.nn.Parameter(q.clone())])
+        with pytest.raises(ValueError, match="layout"):
+            opt.load_state_dict(saved(p))
+        assert not opt.state
+    for name, change in (("exp_avg_scale", lambda x: x[:-1]), ("exp_avg_sq_scale", lambda x: x.double()),
+                         ("exp_avg", lambda x: x.float()), ("exp_avg_sq", lambda x: x.view(torch.uint8))):
+        state = saved(torch.nn.Parameter(w.clone()))
+        state["state"][0][name] = change(state["state"][0][name])
+        with pytest.raises(ValueError, match=name):
+            FusedAdam8bit([torch.nn.Parameter(w.clone())]).load_state_dict(state)
+    column = torch.randn(200, 1)
+    other = torch.nn.Parameter(column.as_strided((200, 1), (1, 7)))
+    state = saved(torch.nn.Parameter(column.clone()))
+    opt = FusedAdam8bit([other])
+    opt.load_state_dict(state)
+    other.grad = torch.ones(200, 1)
+    opt.step()
+    assert opt.state[other]["exp_avg"].shape == (200, 1)
