@@ -413,27 +413,31 @@ void adam_8bit(TensorLists& lists, const std::vector<long>& ordinals, const Adam
   const auto type = lists[1][0].scalar_type();
   const at::DeviceGuard guard(device);
   auto stream = current_stream();
+  // all are looked at before the first launch: a step that is refused has changed no tensor
+  for (size_t t = 0; t < count; ++t) {
+    // a gradient of another layout is met in the param's order; the copy lives until the launches are under way
+    if (lists[0][t].strides() != lists[1][t].strides() && lists[0][t].numel() > 1)
+      lists[0][t] = at::empty_like(lists[1][t]).copy_(lists[0][t]);
+    const long n = lists[1][t].numel(), blocks = (n + A8_SCALE_BLOCK - 1) / A8_SCALE_BLOCK;
+    for (size_t d = 0; d < lists.size(); ++d) {
+      const auto& x = lists[d][t];
+      const bool scales = d == 3 || d == 5;
+      TORCH_CHECK(x.device() == device, "multi_tensor_adam_8bit: tensors on more than one device");
+      TORCH_CHECK(x.numel() == (scales ? blocks : n), "multi_tensor_adam_8bit: size mismatch within tuple");
+      TORCH_CHECK(x.is_non_overlapping_and_dense(), "multi_tensor_adam_8bit: tensor not dense/contiguous");
+      TORCH_CHECK(scales || n <= 1 || x.strides() == lists[1][t].strides(),
+                  "multi_tensor_adam_8bit: layout mismatch within tensor tuple");
+      const auto want = d <= 1 ? type : d == 2 || d == 4 ? at::kFloat8_e4m3fn : at::kFloat;
+      TORCH_CHECK(x.scalar_type() == want, "multi_tensor_adam_8bit: list ", d, " must be ", want, ", got ", x.scalar_type());
+    }
+  }
   Adam8Meta meta;
   size_t t = 0;
   while (t < count) {
     int nt = 0;
     long chunks = 0;
     while (t < count && nt < A8_TENSORS) {
-      // a gradient of another layout is met in the param's order; the copy lives until the launch is under way
-      if (lists[0][t].strides() != lists[1][t].strides() && lists[0][t].numel() > 1)
-        lists[0][t] = at::empty_like(lists[1][t]).copy_(lists[0][t]);
-      const long n = lists[1][t].numel(), blocks = (n + A8_SCALE_BLOCK - 1) / A8_SCALE_BLOCK;
-      for (size_t d = 0; d < lists.size(); ++d) {
-        const auto& x = lists[d][t];
-        const bool scales = d == 3 || d == 5;
-        TORCH_CHECK(x.device() == device, "multi_tensor_adam_8bit: tensors on more than one device");
-        TORCH_CHECK(x.numel() == (scales ? blocks : n), "multi_tensor_adam_8bit: size mismatch within tuple");
-        TORCH_CHECK(x.is_non_overlapping_and_dense(), "multi_tensor_adam_8bit: tensor not dense/contiguous");
-        TORCH_CHECK(scales || n <= 1 || x.strides() == lists[1][t].strides(),
-                    "multi_tensor_adam_8bit: layout mismatch within tensor tuple");
-        const auto want = d <= 1 ? type : d == 2 || d == 4 ? at::kFloat8_e4m3fn : at::kFloat;
-        TORCH_CHECK(x.scalar_type() == want, "multi_tensor_adam_8bit: list ", d, " must be ", want, ", got ", x.scalar_type());
-      }
+      const long n = lists[1][t].numel();
       if (n) {
         meta.g[nt] = lists[0][t].data_ptr();
         meta.p[nt] = lists[1][t].data_ptr();

@@ -565,3 +565,20 @@ def test_a_capture_needs_capturable():
             opt.step()
     assert opt.param_groups[0]["step"] == 1
     opt.step()
+
+
+def test_a_refused_step_changes_nothing():
+    """A tensor that does not fit, behind those of a first launch: found before any is stepped."""
+    pa, ga = make([(10,)] * 60, torch.float32, device="cuda")
+    opt = FusedAdam8bit(pa, lr=1e-2)
+    ga(0)
+    opt.step()
+    good = opt.state[pa[55]]["exp_avg_scale"]
+    opt.state[pa[55]]["exp_avg_scale"] = torch.zeros(5, device="cuda")
+    before = [p.detach().clone() for p in pa] + [opt.state[p]["exp_avg"].clone() for p in pa]
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        opt.step()
+    for b, a in zip(before, pa + [opt.state[p]["exp_avg"] for p in pa]):
+        assert torch.equal(b.view(torch.uint8), a.detach().view(torch.uint8))
+    opt.state[pa[55]]["exp_avg_scale"] = good
+    opt.step()
