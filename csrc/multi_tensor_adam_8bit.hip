@@ -26,6 +26,7 @@
 
 #include <c10/core/DeviceGuard.h>
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -41,6 +42,7 @@ constexpr int A8_PER_LANE = 4;         // elements: 32 lanes have a block of 128
 constexpr int A8_SCALE_BLOCK = 128;    // elements of one scale
 constexpr int A8_CHUNK = A8_BLOCK * A8_PER_LANE;  // elements of a workgroup
 constexpr int A8_TENSORS = 48;         // of one launch: 48 * 72 B of kernel arguments
+constexpr long A8_SIDE = 1 << 23;      // workgroups along a grid's x
 constexpr float E4M3_MAX = 448.f;
 
 struct Adam8Meta {
@@ -264,15 +266,18 @@ __global__ void __launch_bounds__(A8_BLOCK) adam_8bit_kernel(Adam8Meta meta, Ada
   if (a.lr_ptr) a.lr = *a.lr_ptr;
   const float unscale = a.inv_scale ? *a.inv_scale : 1.f;
 
+  // a grid counts threads in 32 bits along each side: the chunks of more than 2^33 elements go on along y, and the last
+  // row of workgroups may lie behind the last tensor, where no lane has an element
+  const int chunk = (int)(blockIdx.y * gridDim.x + blockIdx.x);
   int t = 0;
   {
     int hi = meta.ntensors - 1;
     while (t < hi) {
       const int mid = (t + hi + 1) >> 1;
-      if (meta.chunk_prefix[mid] <= (int)blockIdx.x) t = mid; else hi = mid - 1;
+      if (meta.chunk_prefix[mid] <= chunk) t = mid; else hi = mid - 1;
     }
   }
-  const long n = meta.sizes[t], base = (long)((int)blockIdx.x - meta.chunk_prefix[t]) * A8_CHUNK;
+  const long n = meta.sizes[t], base = (long)(chunk - meta.chunk_prefix[t]) * A8_CHUNK;
   T* gp = (T*)meta.g[t];
   T* pp = (T*)meta.p[t];
   float* wp = (float*)meta.master[t];
@@ -450,8 +455,6 @@ void adam_8bit(TensorLists& lists, const std::vector<long>& ordinals, const Adam
         meta.ordinal[nt] = (int)ordinals[t];
         meta.chunk_prefix[nt] = (int)chunks;
         chunks += (n + A8_CHUNK - 1) / A8_CHUNK;
-        // a launch's threads are counted in 32 bits
-        TORCH_CHECK(chunks < (1L << 32) / A8_BLOCK, "multi_tensor_adam_8bit: too many elements in one launch");
         ++nt;
       }
       ++t;
@@ -459,11 +462,12 @@ void adam_8bit(TensorLists& lists, const std::vector<long>& ordinals, const Adam
     if (!nt) continue;
     meta.chunk_prefix[nt] = (int)chunks;
     meta.ntensors = nt;
+    const dim3 grid((unsigned)std::min(chunks, A8_SIDE), (unsigned)((chunks + A8_SIDE - 1) / A8_SIDE));
     APEX_DISPATCH_FLOAT_HALF_BF(type, "multi_tensor_adam_8bit", ([&] {
       if (master) {
-        hipLaunchKernelGGL((adam_8bit_kernel<scalar_t, true>), dim3((unsigned)chunks), dim3(A8_BLOCK), 0, stream, meta, args);
+        hipLaunchKernelGGL((adam_8bit_kernel<scalar_t, true>), grid, dim3(A8_BLOCK), 0, stream, meta, args);
       } else {
-        hipLaunchKernelGGL((adam_8bit_kernel<scalar_t, false>), dim3((unsigned)chunks), dim3(A8_BLOCK), 0, stream, meta, args);
+        hipLaunchKernelGGL((adam_8bit_kernel<scalar_t, false>), grid, dim3(A8_BLOCK), 0, stream, meta, args);
       }
     }()));
     HIP_CHECK(hipGetLastError());

@@ -582,3 +582,23 @@ def test_a_refused_step_changes_nothing():
         assert torch.equal(b.view(torch.uint8), a.detach().view(torch.uint8))
     opt.state[pa[55]]["exp_avg_scale"] = good
     opt.step()
+
+
+def test_more_elements_than_one_grid_has_threads_for():
+    """9 params of 2^31 elements: 2^34 and more, four a thread. The first step is lr everywhere (m over the root of v is 1),
+    and a moment is the same code for every element: each is its block's largest."""
+    n = 2 ** 31
+    grad = torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda")
+    params = [torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda")) for _ in range(9)]
+    for p in params:
+        p.grad = grad
+    opt = FusedAdam8bit(params, lr=2.0 ** -7)
+    opt.step()
+    for p in params:
+        # a step of 2^-7 (1 - 2 half steps and eps / 0.5) is 2^-7 in bf16
+        assert p.detach().min() == p.detach().max() == -(2.0 ** -7)
+        for k in ("exp_avg", "exp_avg_sq"):
+            top = opt.state[p][k].view(torch.uint8)
+            assert top.min() == top.max() == 126
+            scale = opt.state[p][k + "_scale"]
+            assert scale.min() == scale.max() > 0
