@@ -257,6 +257,20 @@ def policy_loss(logits, labels, old_log_probs, advantages, ref_log_probs=None, c
     return _ref_policy(lp, *args)
 
 
+class _One(torch.autograd.Function):
+    """exp(x - x) with x's gradient: 1, where x is -inf as well."""
+
+    @staticmethod
+    def forward(ctx, x):
+        one = torch.where(torch.isnan(x), x, 1.0)
+        ctx.save_for_backward(one)
+        return one
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad * ctx.saved_tensors[0]
+
+
 def _ref_policy(lp, labels, old, advantages, by_row, ref, cu_seqlens, count, low, high, kl, temperature, reduction, ignore_index):
     if cu_seqlens is None and labels.dim() == 1:
         owner, inside = torch.zeros_like(labels), torch.ones_like(labels, dtype=torch.bool)
@@ -265,9 +279,12 @@ def _ref_policy(lp, labels, old, advantages, by_row, ref, cu_seqlens, count, low
     on = inside & (labels != ignore_index).view(-1)
     x, owner = lp.reshape(-1)[on], owner[on]
     a = advantages.view(-1)[on] if by_row else advantages[owner]
-    ratio = torch.exp(x - (x.detach() if old is None else old.view(-1)[on]))
-    bound, free = ratio.clamp(1 - low, 1 + high) * a, ratio * a
-    each = -torch.where(free > bound, bound, free)
+    ratio = _One.apply if old is None else lambda z: torch.exp(z - old.view(-1)[on])
+    now = ratio(x.detach())
+    bound = now.clamp(1 - low, 1 + high) * a
+    held = now * a > bound
+    # a token that the clip holds has no gradient: not that of a ratio of inf, times 0, either
+    each = -torch.where(held, bound, ratio(torch.where(held, x.detach(), x)) * a)
     if ref is not None:
         d = ref.view(-1)[on] - x
         each = each + kl * (torch.expm1(d) - d)

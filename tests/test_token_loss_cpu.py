@@ -185,3 +185,26 @@ def test_refusals():
         policy_loss(x, y, ok, torch.zeros(4), grad_scale=1.0, reduction="none")
     with pytest.raises(ValueError, match="token"):
         policy_loss(x[:, :0], y[:, :0], ok[:, :0], torch.zeros(4))
+
+
+def test_a_ratio_that_overflows_and_one_of_nothing():
+    """Where a clip holds a ratio of inf the gradient is 0, as where it holds any other; without old_log_probs the ratio is
+    1, and its gradient that of lp, for a token of probability 0 too."""
+    x = torch.zeros(1, 3, 4)
+    x[0, 0, 1] = -math.inf
+    x.requires_grad_(True)
+    y = torch.tensor([[1, 2, 0]])
+    p = torch.softmax(x.detach(), -1)
+    want = (torch.nn.functional.one_hot(y, 4) - p) / 3  # of the mean of lp
+    for a, reduction in ((1.0, "token"), (-2.0, "sequence"), (0.5, "sum")):
+        adv = torch.full((1,), a)
+        loss, lp = policy_loss(x, y, None, adv, reduction=reduction)
+        n = 3 if reduction != "sum" else 1
+        assert lp[0, 0] == -math.inf and loss == -a * 3 / n
+        torch.testing.assert_close(torch.autograd.grad(loss, x)[0], -a * want * 3 / n, rtol=0, atol=8 * 2 ** -24)
+    # exp(lp - old) is inf, in the middle token held at 1.2
+    old = torch.tensor([[0.0, -200.0, -1.3]])
+    loss, _ = policy_loss(x, y, old, torch.ones(1), reduction="none")
+    assert loss[0, 0] == 0 and abs(loss[0, 1].item() + 1.2) < 4 * 2 ** -24
+    dx = torch.autograd.grad(loss, x, torch.ones(1, 3))[0]
+    assert (dx[0, :2] == 0).all() and torch.isfinite(dx).all() and dx[0, 2].abs().sum() > 0

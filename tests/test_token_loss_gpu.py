@@ -546,3 +546,20 @@ def test_rows_beyond_32_bits():
     lp = oracle.log_probs(l64, y[-2:].cpu())
     near(dx[-2:], torch.autograd.grad(lp.sum(), l64)[0], oracle.grad_bound(last, y[-2:].cpu(), torch.ones(2), torch.bfloat16))
     assert not dx[:-2].any()
+
+
+def test_a_ratio_that_overflows_and_one_of_nothing():
+    """The clip's and the kernel's own sides of an infinite ratio, and of a token of probability 0, as the CPU path has them."""
+    x = torch.zeros(1, 3, 4)
+    x[0, 0, 1] = -math.inf
+    y = torch.tensor([[1, 2, 0]])
+    for old in (None, torch.tensor([[0.0, -200.0, -1.3]])):
+        for scale in (None, 1.0):
+            out = []
+            for device in ("cpu", "cuda"):
+                z = x.to(device).requires_grad_(True)
+                loss, lp = policy_loss(z, y.to(device), None if old is None else old.to(device), torch.ones(1, device=device), grad_scale=scale)
+                out.append([loss.detach().cpu(), lp.cpu(), torch.autograd.grad(loss, z)[0].cpu()])
+            for a, b in zip(*out):
+                assert not torch.isnan(a).any()
+                torch.testing.assert_close(a, b, rtol=0, atol=8 * 2 ** -24)
