@@ -835,7 +835,7 @@ Sequences sequences_of(const at::Tensor& labels, const c10::optional<at::Tensor>
     TORCH_CHECK(cu->numel() == count + 1, "token_loss: cu_seqlens has one value more than sequences");
     s.cu = cu->data_ptr<int>();
   } else {
-    TORCH_CHECK(count > 0 && labels.numel() % count == 0, "token_loss: rows do not divide into sequences");
+    TORCH_CHECK(count > 0 ? labels.numel() % count == 0 : labels.numel() == 0, "token_loss: rows do not divide into sequences");
   }
   return s;
 }

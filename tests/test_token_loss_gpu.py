@@ -563,3 +563,19 @@ def test_a_ratio_that_overflows_and_one_of_nothing():
             for a, b in zip(*out):
                 assert not torch.isnan(a).any()
                 torch.testing.assert_close(a, b, rtol=0, atol=8 * 2 ** -24)
+
+
+def test_no_sequences():
+    """An empty batch has no log-probabilities and an empty gradient, as on the CPU."""
+    for device in ("cpu", "cuda"):
+        x = torch.zeros(0, 3, 7, device=device, requires_grad=True)
+        y = torch.zeros(0, 3, dtype=torch.long, device=device)
+        for average in (False, True):
+            out = sequence_log_probs(x, y, average=average)
+            assert out.shape == (0,) and out.dtype == torch.float32
+            assert torch.autograd.grad(out.sum(), x)[0].shape == x.shape
+        assert token_log_probs(x, y).shape == (0, 3)
+        with pytest.raises(ValueError, match="needs"):
+            preference_loss(x, y, torch.zeros(0, device=device))
+        with pytest.raises(ValueError, match="needs"):
+            policy_loss(x, y, None, torch.zeros(0, device=device))
