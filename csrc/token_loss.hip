@@ -724,7 +724,7 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
     put_zeros();
     return;
   }
-  const Gradient d{f, w.m, l2, c.hi};
+  const Gradient d{f, w.m, l2, c.hi + c.lo};  // the base rounded to nearest, as row_grad_kernel has it
 #pragma unroll
   for (int u = 0; u < NP; ++u)
     if (u < NP - 2 || has[u - (NP - 2)]) {

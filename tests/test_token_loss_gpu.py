@@ -579,3 +579,17 @@ def test_no_sequences():
             preference_loss(x, y, torch.zeros(0, device=device))
         with pytest.raises(ValueError, match="needs"):
             policy_loss(x, y, None, torch.zeros(0, device=device))
+
+
+@pytest.mark.parametrize("t", [0.7, 1.0, 1.3])
+def test_both_ways_of_the_policy_gradient_round_alike(t):
+    """Logits far apart, where an exponent's base that is off shows. A row has one pack a lane both ways, so its sum and
+    then each step of its gradient are the same: so are all bits."""
+    x = (torch.randn(4, 16, 256, generator=torch.Generator().manual_seed(7)) * 30).cuda().requires_grad_(True)
+    y = x.detach().argmax(-1)
+    adv, out = torch.ones(4, device="cuda"), []
+    for scale in (None, 1.0):
+        loss, lp = policy_loss(x, y, None, adv, temperature=t, reduction="sum", grad_scale=scale)
+        out.append([lp, torch.autograd.grad(loss, x, torch.ones((), device="cuda"))[0]])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
