@@ -202,7 +202,8 @@ def policy_loss(logits, labels, old_log_probs, advantages, ref_log_probs=None, c
         logits: ``[sequences, length, V]``, or ``[tokens, V]`` with 1-D labels.
         old_log_probs: of the policy that the tokens were drawn from, of the labels' shape (at the same
             ``temperature``); ``None`` if it is this one (``ratio`` is 1, its gradient is that of ``lp``).
-        advantages: of the labels' shape, or ``[sequences]``.
+        advantages: of the labels' shape, or ``[sequences]`` or ``[sequences, 1]``. Of as many packed sequences as tokens
+            ``[sequences]`` is the labels' shape and goes by token: ``[sequences, 1]`` goes by sequence there too.
         ref_log_probs: of the labels' shape; needed where ``kl_coef`` is not 0.
         clip_eps_high: the upper clip, ``clip_eps`` if ``None``.
         reduction: ``"token"``, the mean over all labelled tokens; ``"sequence"``, the mean over all sequences of their
@@ -238,7 +239,7 @@ def policy_loss(logits, labels, old_log_probs, advantages, ref_log_probs=None, c
     old = None if old_log_probs is None else _given(old_log_probs, "old_log_probs", logits, labels.shape)
     ref = None if ref_log_probs is None or not kl_coef else _given(ref_log_probs, "ref_log_probs", logits, labels.shape)
     by_row = advantages.shape == labels.shape
-    advantages = _given(advantages, "advantages", logits, labels.shape, (count,))
+    advantages = _given(advantages, "advantages", logits, labels.shape, (count,), (count, 1))
     if grad_scale is not None:
         if reduction == "none":
             raise ValueError("grad_scale goes with a loss that is one number: not with reduction='none'")
@@ -278,7 +279,7 @@ def _ref_policy(lp, labels, old, advantages, by_row, ref, cu_seqlens, count, low
         owner, inside = _ref_owner(labels, cu_seqlens)
     on = inside & (labels != ignore_index).view(-1)
     x, owner = lp.reshape(-1)[on], owner[on]
-    a = advantages.view(-1)[on] if by_row else advantages[owner]
+    a = advantages.view(-1)[on if by_row else owner]
     ratio = _One.apply if old is None else lambda z: torch.exp(z - old.view(-1)[on])
     now = ratio(x.detach())
     bound = now.clamp(1 - low, 1 + high) * a

@@ -208,3 +208,28 @@ def test_a_ratio_that_overflows_and_one_of_nothing():
     assert loss[0, 0] == 0 and abs(loss[0, 1].item() + 1.2) < 4 * 2 ** -24
     dx = torch.autograd.grad(loss, x, torch.ones(1, 3))[0]
     assert (dx[0, :2] == 0).all() and torch.isfinite(dx).all() and dx[0, 2].abs().sum() > 0
+
+
+def test_advantages_of_as_many_sequences_as_tokens():
+    """[sequences] is the labels' shape there and goes by token; [sequences, 1] goes by sequence whatever their number."""
+    cu = [0, 2, 2, 3, 4, 5]
+    x, y, g = make((5,), 6)
+    y = y.clamp(min=0)
+    adv = torch.randn(5, generator=g)
+    packed = torch.tensor(cu, dtype=torch.int32)
+    old = oracle.log_probs(x.double(), y).float() + 0.1 * torch.randn(5, generator=g)
+    rows = adv[torch.tensor([0, 0, 2, 3, 4])]  # what the sequences' are for the tokens
+    for a, each in ((adv, adv), (adv[:, None], rows)):
+        x64, mine = both(x)
+        want, _ = oracle.policy(x64, y, old, each, cu=cu)
+        got, _ = policy_loss(mine, y, old, a, cu_seqlens=packed)
+        torch.testing.assert_close(got.double(), want, **TOL)
+        wanted, dx = grads(want, x64, got, mine)
+        torch.testing.assert_close(dx, wanted, **TOL)
+    # a padded batch takes it too
+    x, y, g = make((3, 4), 6)
+    a = policy_loss(x, y, None, adv[:3])[0]
+    assert torch.equal(a, policy_loss(x, y, None, adv[:3, None])[0])
+    for bad in (adv[:4, None], adv[None, :3]):
+        with pytest.raises(ValueError, match="advantages"):
+            policy_loss(x, y, None, bad)

@@ -593,3 +593,20 @@ def test_both_ways_of_the_policy_gradient_round_alike(t):
         out.append([lp, torch.autograd.grad(loss, x, torch.ones((), device="cuda"))[0]])
     for a, b in zip(*out):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scale", [None, 1.0])
+def test_advantages_of_as_many_sequences_as_tokens(scale):
+    """[sequences] is the labels' shape there and goes by token; [sequences, 1] goes by sequence: the CPU path's results."""
+    x, y, g = make((5,), 6, torch.float32, ignored=0)
+    adv, cu = torch.randn(5, generator=g), torch.tensor([0, 2, 2, 3, 4, 5], dtype=torch.int32)
+    old = oracle.log_probs(x.double(), y).float() + 0.1 * torch.randn(5, generator=g)
+    for a in (adv, adv[:, None]):
+        out = []
+        for device in ("cpu", "cuda"):
+            z = x.to(device).requires_grad_(True)
+            loss, _ = policy_loss(z, y.to(device), old.to(device), a.to(device), cu_seqlens=cu.to(device), grad_scale=scale)
+            out.append([loss.detach().cpu(), torch.autograd.grad(loss, z)[0].cpu()])
+        for a, b in zip(*out):
+            # losses and slopes of up to 3, in fp32 on both sides
+            torch.testing.assert_close(a, b, rtol=0, atol=64 * 2 ** -24)
