@@ -18,6 +18,7 @@ import torch
 from .._ext import get_ext
 from ..multi_tensor_apply import multi_tensor_applier
 from ..tracing import traced
+from ._scaling import found_inf_and_inv_scale
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -196,11 +197,11 @@ class FusedAdam(torch.optim.Optimizer):
 
         if self.capturable:
             if grad_scaler is not None:
-                scale = grad_scaler._get_scale_async()
-                found_inf = grad_scaler._check_inf_per_device(self)[device]
-                noop = found_inf.to(torch.int32) if found_inf.dtype != torch.int32 else found_inf
-                inv_scale = scale.double().reciprocal().float()
+                found_inf, inv_scale = found_inf_and_inv_scale(self, grad_scaler)
+                noop = found_inf[device].to(torch.int32)
             else:
+                inv_scale = None
+            if inv_scale is None:
                 inv_scale = torch.ones(1, dtype=torch.float32, device=device)
             lr = group["lr"].to(device) if group["lr"].device != device else group["lr"]
             step_t = group["step"]

@@ -14,10 +14,10 @@ moments before they are rounded. Device path: csrc/multi_tensor_adam_8bit.hip. C
 import math
 
 import torch
-from torch.amp.grad_scaler import OptState
 
 from .._ext import get_ext
 from ..tracing import traced
+from ._scaling import found_inf_and_inv_scale
 
 BLOCK = 128  # elements of one scale
 _E4M3_MAX = 448.0
@@ -218,7 +218,9 @@ class FusedAdam8bit(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
 
-        founds, unscale = self._asked(grad_scaler)
+        founds = unscale = None
+        if self.capturable and grad_scaler is not None:
+            founds, unscale = found_inf_and_inv_scale(self, grad_scaler)
         first = 0  # a tensor's place in the optimizer is part of its random numbers
         for group in self.param_groups:
             params = group["params"]
@@ -256,15 +258,6 @@ class FusedAdam8bit(torch.optim.Optimizer):
                         self._step_ref(group, place, inv_scale, grad, p, *(state[name] for name in names))
         return loss
 
-    def _asked(self, grad_scaler):
-        """What GradScaler found on each device (it looks at all gradients: once a step), and 1 / scale."""
-        if grad_scaler is None or not self.capturable:
-            return None, None
-        state = grad_scaler._per_optimizer_states[id(self)]
-        if state["stage"] is OptState.UNSCALED:  # unscale_ has divided the gradients, and kept what it found
-            return list(state["found_inf_per_device"].values()), None
-        return list(grad_scaler._check_inf_per_device(self).values()), grad_scaler._get_scale_async().double().reciprocal().float()
-
     def _count(self, group, founds, inv_scale):
         """Advances the group's step; what GradScaler has for it, on its device."""
         device = group["params"][0].device
@@ -282,7 +275,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
             group["step"].add_(1)  # in place: a hipGraph's replay has to see it
             return None, None
         # a gradient on any device that is not finite skips the step on all
-        found = [f.to(device=device, dtype=torch.float32) for f in founds]
+        found = [f.to(device=device, dtype=torch.float32) for f in founds.values()]
         found_inf = found[0] if len(found) == 1 else torch.stack(found).amax(0)
         group["step"].add_((found_inf == 0).to(torch.int32))
         return found_inf, inv_scale if inv_scale is None else inv_scale.to(device)
