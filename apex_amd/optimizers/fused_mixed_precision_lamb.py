@@ -12,6 +12,7 @@ import torch
 
 from .._ext import get_ext
 from ..multi_tensor_apply import multi_tensor_applier
+from ._scaling import found_inf_and_inv_scale
 
 
 class FusedMixedPrecisionLamb(torch.optim.Optimizer):
@@ -84,11 +85,11 @@ class FusedMixedPrecisionLamb(torch.optim.Optimizer):
 
         # Scale handling (device tensors; graph-safe).
         if grad_scaler is not None:
-            found_inf = grad_scaler._check_inf_per_device(self)[device]
-            scale = grad_scaler._get_scale_async()
-            inv_scale = scale.double().reciprocal().float()
+            found_inf, inv_scale = found_inf_and_inv_scale(self, grad_scaler)
+            found_inf = found_inf[device]
         else:
-            found_inf = torch.zeros(1, dtype=torch.float32, device=device)
+            found_inf, inv_scale = torch.zeros(1, dtype=torch.float32, device=device), None
+        if inv_scale is None:
             inv_scale = torch.ones(1, dtype=torch.float32, device=device)
 
         # Collect all grads for global norm.
