@@ -895,12 +895,13 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
     };
     // A block's cost is that of its start and of its join, which grow with its waves, and of its passes one after
     // another. 8192 rows of 2048 bf16: 9.9 us by 64 lanes, 19.9 by 256; of 8192: 24.0 by 128, 28.7 by 256; of 32000:
-    // 86.9 by 256, 103 by 512; of 131072: 327 by 256, 310 by 512. Few rows wait for their passes, not for room: 512
-    // rows of 8192 5.5 by 128, 5.0 by 256.
+    // 86.9 by 256, 103 by 512; of 131072: 327 by 256, 310 by 512. Up to 512 rows, two for a compute unit, wait for their
+    // passes, not for room: 256 rows of 20000 6.6 by 256, 5.6 by 512, 512 rows 7.6 and 7.5, 640 rows 8.9 and 9.8; of 4800
+    // 4.3 and 4.2, 4.7 and 4.8, 5.0 and 6.7.
     using std::integral_constant;
     if (packs <= 512) launch(integral_constant<int, 64>{});
     else if (packs <= 1536 && rows >= 1024) launch(integral_constant<int, 128>{});
-    else if (packs < (rows >= 1024 ? 8192 : 3000)) launch(integral_constant<int, 256>{});
+    else if (rows > 512 && packs < 8192) launch(integral_constant<int, 256>{});
     else launch(integral_constant<int, 512>{});
   }()));
   HIP_CHECK(hipGetLastError());
