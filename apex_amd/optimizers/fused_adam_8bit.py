@@ -221,6 +221,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
         founds = unscale = None
         if self.capturable and grad_scaler is not None:
             founds, unscale = found_inf_and_inv_scale(self, grad_scaler)
+        masters = self.master_weights
         first = 0  # a tensor's place in the optimizer is part of its random numbers
         for group in self.param_groups:
             params = group["params"]
@@ -236,7 +237,7 @@ class FusedAdam8bit(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     self._init_state(p, state)
-                if self.master_weights and "master_param" not in state and p.dtype != torch.float32:
+                if masters and "master_param" not in state and p.dtype != torch.float32:
                     self._init_master(p, state)  # new, or loaded from a checkpoint without
                 key = p.device, p.dtype, "master_param" in state
                 row = place, grad, p, state
