@@ -152,9 +152,56 @@ struct Base {
   __device__ __forceinline__ float exp(float d) const { return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo)); }
 };
 
-// m = max x, s = sum exp((x - m) / T), over what has been added
+// op over each N neighbouring lanes, on all of them, without LDS: exchanges within
+// quads, mirrored halves and rows of 16, then between rows and halves of the wave.
+// Lanes of a group hold the same value before they meet another group, so that a
+// mirror is an exchange.
+template <int CTRL>
+__device__ __forceinline__ float lane_across(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double lane_across(double v) {
+  return __hiloint2double(__builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xF, 0xF, true),
+                          __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xF, 0xF, true));
+}
+template <bool HALVES>
+__device__ __forceinline__ void swap_rows(unsigned v, unsigned& a, unsigned& b) {
+  const auto r = HALVES ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  a = r[0];
+  b = r[1];
+}
+template <bool HALVES, typename F>
+__device__ __forceinline__ float over_rows(float v, F op) {
+  unsigned a, b;
+  swap_rows<HALVES>(__float_as_uint(v), a, b);
+  return op(__uint_as_float(a), __uint_as_float(b));
+}
+template <bool HALVES, typename F>
+__device__ __forceinline__ double over_rows(double v, F op) {
+  unsigned ah, bh, al, bl;
+  swap_rows<HALVES>(__double2hiint(v), ah, bh);
+  swap_rows<HALVES>(__double2loint(v), al, bl);
+  return op(__hiloint2double(ah, al), __hiloint2double(bh, bl));
+}
+template <int N, typename V, typename F>
+__device__ __forceinline__ V over_lanes(V v, F op) {
+  if constexpr (N >= 2) v = op(v, lane_across<0xB1>(v));    // quad_perm 1,0,3,2
+  if constexpr (N >= 4) v = op(v, lane_across<0x4E>(v));    // quad_perm 2,3,0,1
+  if constexpr (N >= 8) v = op(v, lane_across<0x141>(v));   // row_half_mirror
+  if constexpr (N >= 16) v = op(v, lane_across<0x140>(v));  // row_mirror
+  if constexpr (N >= 32) v = over_rows<false>(v, op);
+  if constexpr (N >= 64) v = over_rows<true>(v, op);
+  return v;
+}
+
+// m = max x, s = sum exp((x - m) / T), over what has been added. A pack's few terms
+// are added in 32 bits, packs and lanes in 64: half a step off in each of some
+// twenty sums of every row shows in the small difference of two answers' hundreds
+// of log-probabilities.
 struct Running {
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY;
+  double s = 0;
   // differences are taken from 0 where all so far is -inf: exp of -inf is 0
   __device__ __forceinline__ float origin() const { return m == -INFINITY ? 0.f : m; }
   __device__ __forceinline__ void raise(float top, Base c) {
@@ -163,32 +210,35 @@ struct Running {
       m = top;
     }
   }
-  __device__ __forceinline__ void join(float mb, float sb, Base c) {
+  __device__ __forceinline__ void join(float mb, double sb, Base c) {
     const float ma = m;
     m = fmaxf(m, mb);
     const float o = origin();
     s = s * c.exp(ma - o) + sb * c.exp(mb - o);
   }
+  // over each N neighbouring lanes, on all of them
+  template <int N>
+  __device__ __forceinline__ void join_lanes(Base c) {
+    const float ma = m;
+    m = over_lanes<N>(m, [](float a, float b) { return fmaxf(a, b); });
+    s = over_lanes<N>(s * c.exp(ma - origin()), [](double a, double b) { return a + b; });
+  }
 };
 
 template <int BLOCK>
-__device__ __forceinline__ Running block_join(Running w, Base c, float* smem) {
-#pragma unroll
-  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1)
-    w.join(__shfl_xor(w.m, off), __shfl_xor(w.s, off), c);
+__device__ __forceinline__ Running block_join(Running w, Base c, double* smem) {
   constexpr int NW = BLOCK / WAVE_SIZE;
+  w.join_lanes<WAVE_SIZE>(c);
+  if (NW == 1) return w;
   if ((threadIdx.x & (WAVE_SIZE - 1)) == 0) {
     smem[2 * (threadIdx.x / WAVE_SIZE)] = w.m;
     smem[2 * (threadIdx.x / WAVE_SIZE) + 1] = w.s;
   }
   __syncthreads();
-  Running all;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) all.m = fmaxf(all.m, smem[2 * i]);
-  const float o = all.origin();
-#pragma unroll
-  for (int i = 0; i < NW; ++i) all.s = fmaf(smem[2 * i + 1], c.exp(smem[2 * i] - o), all.s);
-  return all;
+  w.m = (float)smem[2 * (threadIdx.x & (NW - 1))];
+  w.s = smem[2 * (threadIdx.x & (NW - 1)) + 1];
+  w.join_lanes<NW>(c);
+  return w;
 }
 
 // U packs into the running maximum and sum: one rescaling for all of them
@@ -204,10 +254,15 @@ __device__ __forceinline__ void take(Running& w, const Pack<T>* v, Base c) {
   const float o = w.origin();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float part = 0.f;
+    float part[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) part += c.exp(to_float(v[u].a[j]) - o);
-    w.s += part;
+    for (int j = 0; j < W; ++j) part[j] = c.exp(to_float(v[u].a[j]) - o);
+    // by halves: a term meets two or three sums
+#pragma unroll
+    for (int half = W / 2; half > 0; half /= 2)
+#pragma unroll
+      for (int j = 0; j < half; ++j) part[j] += part[j + half];
+    w.s += part[0];
   }
 }
 
@@ -228,9 +283,9 @@ struct RowOut {
     else lp[row] = value;
   }
   __device__ __forceinline__ void put(long row, float x, Running w, double inv_t) const {
-    const float l2 = log2f(w.s);
+    const float l2 = log2f((float)w.s);
     stats[row] = make_float2(w.m, l2);
-    if (lp64) lp64[row] = (double)(x - w.m) * inv_t - log((double)w.s);
+    if (lp64) lp64[row] = (double)(x - w.m) * inv_t - log(w.s);
     else lp[row] = log_prob(x, w, inv_t, l2);
   }
 };
@@ -263,7 +318,7 @@ template <typename T, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) row_stats_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V,
     long rows, Base c, double inv_t, RowOut out, int* __restrict__ arrived) {
-  __shared__ float smem[2 * (BLOCK / WAVE_SIZE)];
+  __shared__ double smem[2 * (BLOCK / WAVE_SIZE)];
   constexpr int W = Pack<T>::width;
   if (arrived && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // for the kernel after this one
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -310,7 +365,7 @@ template <typename T>
 __global__ void __launch_bounds__(PART_BLOCK) row_part_kernel(
     const T* __restrict__ logits, Rows where, const long* __restrict__ labels, long ignore, long V, Base c,
     float2* __restrict__ parts, int* __restrict__ arrived) {
-  __shared__ float smem[2 * (PART_BLOCK / WAVE_SIZE)];
+  __shared__ double smem[2 * (PART_BLOCK / WAVE_SIZE)];
   constexpr int W = Pack<T>::width;
   const long row = blockIdx.y, whole = V / W;
   if (arrived && blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0) *arrived = 0;  // for the kernel after the next
@@ -331,7 +386,7 @@ __global__ void __launch_bounds__(PART_BLOCK) row_part_kernel(
     w.s += c.exp(f - w.origin());
   }
   w = block_join<PART_BLOCK>(w, c, smem);
-  if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float2(w.m, w.s);
+  if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float2(w.m, (float)w.s);
 }
 
 template <typename T>
@@ -349,8 +404,7 @@ __global__ void __launch_bounds__(WAVE_SIZE) row_join_kernel(
     const float2 part = parts[row * count + i];
     w.join(part.x, part.y, c);
   }
-#pragma unroll
-  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) w.join(__shfl_xor(w.m, off), __shfl_xor(w.s, off), c);
+  w.join_lanes<WAVE_SIZE>(c);
   if (threadIdx.x == 0) out.put(row, xy, w, inv_t);
 }
 
@@ -668,7 +722,7 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
     Base c, double inv_t, Sequences seqs, long count, Policy policy, bool weight_by_sequence,
     const float* __restrict__ weights, const float* __restrict__ applied, float* __restrict__ lp_out,
     float* __restrict__ losses, T* __restrict__ grad) {
-  __shared__ float smem[2 * (BLOCK / WAVE_SIZE)];
+  __shared__ double smem[2 * (BLOCK / WAVE_SIZE)];
   constexpr int W = Pack<T>::width;
   const long row = first_row + blockIdx.x;
   const long y = labels[row];
@@ -707,7 +761,7 @@ __global__ void __launch_bounds__(BLOCK, 4) policy_at_once_kernel(
   w.raise(to_float(xt), c);
   w.s += c.exp(to_float(xt) - w.origin());
   w = block_join<BLOCK>(w, c, smem);
-  const float l2 = log2f(w.s), lp = log_prob(valid ? to_float(xy) : NAN, w, inv_t, l2);
+  const float l2 = log2f((float)w.s), lp = log_prob(valid ? to_float(xy) : NAN, w, inv_t, l2);
   float f = 0.f, loss = 0.f;
   const long s = owner_of(seqs, count, row);
   if (s >= 0) {

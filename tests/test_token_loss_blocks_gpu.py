@@ -129,3 +129,22 @@ def test_policy_at_once_in_each_tier(packs, dtype):
     dx = grad_of(loss, xg, torch.tensor(64.0))
     bound = oracle.grad_bound(x, y, size * 16, dtype) + (off * 16).unsqueeze(-1)
     near(dx, torch.autograd.grad(want, x64)[0] * 64, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_row_sum_keeps_what_is_far_under_its_largest_term(dtype):
+    """One term of 1 and 131071 of 2^-27, which fp32 loses where it adds packs of them to the 1: some 2e-6 in each row's
+    log-probability. The small terms are off by 8 half steps of fp32 of their sum (1e-3) together. The pack that holds
+    the 1 is added in fp32: three sums of a little over 1, each off by at most half a step of it, 2^-24."""
+    x = torch.full((140, 131072), -18.75).to(dtype)
+    x[:, 0] = 0
+    y = torch.zeros(140, 1, dtype=torch.long)
+    lp = -torch.logsumexp(x[0].double(), -1)
+    xg = x.cuda().view(140, 1, -1).requires_grad_(True)
+    ref = lp.float().expand(140).contiguous()
+    _, chosen, rejected = preference_loss(xg, y.cuda(), ref.cuda(), beta=1.0)
+    want = lp - ref.double()
+    near(torch.cat([chosen, rejected]), want, 3 * U + 8 * U * lp.abs() + U * want.abs())
+    # one in 32 bits takes the sum rounded once more, and its log2
+    for got in (token_log_probs(xg, y.cuda()), policy_loss(xg, y.cuda(), None, torch.ones(140, device="cuda"), grad_scale=1.0)[1]):
+        near(got, lp.expand(140, 1), torch.tensor(3 * U + 4 * U))
