@@ -116,7 +116,8 @@ class FusedAdam8bit(torch.optim.Optimizer):
     checkpoint without masters, ``master_weights`` makes them from the params in the first step; without it, a
     checkpoint's are left out.
 
-    Unlike :class:`FusedAdam` with ``capturable``, gradients are left as they are (not overwritten unscaled), and a
+    State is made in a param's first step, which cannot be captured; without ``capturable`` none can. Unlike
+    :class:`FusedAdam` with ``capturable``, gradients are left as they are (not overwritten unscaled), and a
     step that GradScaler skips does not count.
     """
 

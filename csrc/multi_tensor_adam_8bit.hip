@@ -20,7 +20,7 @@
 //
 // What bounds it: HBM. Per element of fp32 weights 12 B (g, p in and out) + 4 B
 // of moments + 0.125 B of scales, against 28 B with fp32 moments. 682M bf16
-// weights with masters (16.1 B each): 1.90 ms, 5.8 TB/s; 216M fp32 0.60 ms.
+// weights with masters (16.1 B each): 1.89 ms, 5.8 TB/s; 216M fp32 0.60 ms.
 #include "amp_C.h"
 #include "multi_tensor_apply.h"
 
@@ -33,10 +33,11 @@ namespace {
 
 // Each lane has four neighbouring elements and is done: every load and store of a
 // wave is one piece without gaps, whatever the type, and may go past the caches.
-// With eight a lane (two loads of 16 bytes, 32 apart, for fp32) 682M bf16 weights
-// with masters took 2025 us and 216M fp32 weights 634 us, with four 1942 and
-// 587; with 1024 threads 2051 and 631; workgroups that went on to a second to
-// eighth part took 5 to 15% longer, for nothing was on its way while they rounded.
+// With eight a lane (two loads of 16 bytes, 32 apart, for fp32) the same took 4% and
+// 8% longer; workgroups that went on to a second to eighth part 5 to 15%, for nothing
+// was on its way while they rounded. 682M bf16 weights with masters and 216M fp32
+// weights take 1875 and 600 us by 256 threads, 1895 and 604 by 128, 1975 and 625 by
+// 512, 2045 and 655 by 1024.
 constexpr int A8_BLOCK = 256;          // threads
 constexpr int A8_PER_LANE = 4;         // elements: 32 lanes have a block of 128
 constexpr int A8_SCALE_BLOCK = 128;    // elements of one scale
@@ -71,8 +72,8 @@ struct Adam8Args {
   const int* step_ptr;
 };
 
-// Multiply-xorshift mixing of 32 bits; the odd multipliers are the leading
-// fractional bits of the golden ratio and of the root of 3.
+// Multiply-xorshift mixing of 32 bits; the odd multipliers are the largest prime up
+// to 2^32 over the golden ratio, and the leading fractional bits of the root of 3.
 __device__ __forceinline__ unsigned mix32(unsigned x) {
   x ^= x >> 16;
   x *= 0x9E3779B1u;

@@ -14,7 +14,7 @@
 //
 // What bounds them: HBM. Forward reads the labelled rows once (32768 x 50304 bf16,
 // 18938 labelled: 281 us, 6.8 TB/s), backward reads them once more and writes the
-// whole gradient (870 us, 6.0 TB/s; a large copy by the library moves 5.0). The
+// whole gradient (880 us, 5.9 TB/s; a large copy by the library moves 5.0). The
 // second read is the price of a coefficient that hangs on all rows; where it does
 // not, policy_loss can hold a row in registers between its two uses.
 #include "common.h"
@@ -682,8 +682,8 @@ __global__ void __launch_bounds__(BLOCK) policy_kernel(
 // ---------------- policy loss and gradient at once ----------------
 // Where the gradient of the loss is known beforehand, a row's logits are read
 // once: a block holds them in registers from the first use to the second. 4096 x
-// 131072 bf16 (2550 labelled): 334 us, 5.2 TB/s, one row a compute unit; 11920 x
-// 50304, all labelled: 423 us, 5.7 TB/s, against 591 in two passes. Blocks that
+// 131072 bf16 (2550 labelled): 336 us, 5.2 TB/s, one row a compute unit; 11920 x
+// 50304, all labelled: 431 us, 5.6 TB/s, against 591 in two passes. Blocks that
 // stay and load the next row into each pack's registers as soon as that is
 // written are slower (16000 wide 437 us for 369): their 16 packs, two rows'
 // addresses and the floats in between leave no room for a second row's block.
@@ -928,9 +928,9 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
   APEX_DISPATCH_FLOAT_HALF_BF(logits.scalar_type(), "token_loss", ([&] {
     const auto* x = (const scalar_t*)logits.data_ptr();
     const long packs = V / Pack<scalar_t>::width;
-    // Up to 64 rows of 128 KB and more leave most of the chip without work: one to 64 rows of 131072 bf16 take 10.4
-    // to 11.5 us by blocks of a row each, 5.7 to 10.1 in parts. At half that length the second launch costs what it
-    // saves.
+    // Up to 64 rows of 128 KB and more leave most of the chip without work: one to 64 rows of 131072 bf16 take 10.0 to
+    // 12.4 us by blocks of a row each, 5.5 to 9.7 in parts. At half that length, 5.9 to 7.7 and 5.4 to 8.1, the second
+    // launch costs what it saves, and at a quarter more than that.
     if (rows <= 64 && packs >= 8192) {
       const int parts = (int)((packs + PART_PACKS - 1) / PART_PACKS);
       auto room = at::empty({rows * parts, 2}, logits.options().dtype(at::kFloat));
@@ -948,10 +948,10 @@ void launch_stats(at::Tensor logits, const at::Tensor& labels, long ignore, doub
                          x, where, y, ignore, V, rows, c, 1.0 / temperature, out, arrived);
     };
     // A block's cost is that of its start and of its join, which grow with its waves, and of its passes one after
-    // another. 8192 rows of 2048 bf16: 9.9 us by 64 lanes, 19.9 by 256; of 8192: 24.0 by 128, 28.7 by 256; of 32000:
-    // 86.9 by 256, 103 by 512; of 131072: 327 by 256, 310 by 512. Up to 512 rows, two for a compute unit, wait for their
-    // passes, not for room: 256 rows of 20000 6.6 by 256, 5.6 by 512, 512 rows 7.6 and 7.5, 640 rows 8.9 and 9.8; of 4800
-    // 4.3 and 4.2, 4.7 and 4.8, 5.0 and 6.7.
+    // another. 8192 rows of 2048 bf16: 10.3 us by 64 lanes, 14.7 by 128; of 8192: 26.6 by 128, 29.2 by 256; of 32000:
+    // 87 by 256, 105 by 512; of 131072: 330 by 256, 319 by 512. Up to 512 rows, two for a compute unit, wait for their
+    // passes, not for room: 256 rows of 20000 6.4 by 256, 5.4 by 512, 512 rows 7.5 and 7.2, 640 rows 8.6 and 9.2; of 4800
+    // 4.2 and 4.0, 4.5 and 4.6, 4.8 and 6.2.
     using std::integral_constant;
     if (packs <= 512) launch(integral_constant<int, 64>{});
     else if (packs <= 1536 && rows >= 1024) launch(integral_constant<int, 128>{});
