@@ -210,11 +210,11 @@ def policy_loss(logits, labels, old_log_probs, advantages, ref_log_probs=None, c
             tokens' mean (0 for a sequence without one); ``"sum"``; ``"none"``, the loss of each token.
         cu_seqlens: int32 ``[sequences + 1]``, for 1-D labels; tokens outside have no part. Without it, 1-D labels are
             one sequence.
-        grad_scale: a number, or a tensor of one fp32 value on the logits' device, finite and not 0. Where it is given, the forward pass
-            also makes the logits' gradient, for a loss that is going to be multiplied by ``grad_scale`` before
-            ``backward()`` (1 if it is not), and where a row fits a compute unit's registers it reads the logits only
-            once. It keeps that gradient in place of the logits. If another gradient of the loss arrives, the kept one
-            is multiplied by their quotient. The backward pass can then be run once only.
+        grad_scale: a number, or a tensor of one fp32 value on the logits' device, finite and not 0. Where it is given,
+            the forward pass also makes the logits' gradient, for a loss that is going to be multiplied by
+            ``grad_scale`` before ``backward()`` (1 if it is not), and where a row fits a compute unit's registers it
+            reads the logits only once. It keeps that gradient in place of the logits. If another gradient of the loss
+            arrives, the kept one is multiplied by their quotient. The backward pass can then be run once only.
 
     Returns:
         ``(loss, log_probs)``: the loss, differentiable in the logits, and the tokens' log-probabilities, fp32 of the
