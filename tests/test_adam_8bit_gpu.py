@@ -602,3 +602,5 @@ def test_more_elements_than_one_grid_has_threads_for():
             assert top.min() == top.max() == 126
             scale = opt.state[p][k + "_scale"]
             assert scale.min() == scale.max() > 0
+    del params, opt, grad, p, top, scale
+    torch.cuda.empty_cache()
